@@ -168,6 +168,15 @@ _SIGNATURES = {
     "b200_token_gate_rows": ("gated_residual", [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
                                                 c_int, c_int, c_int]),
     "b200_argmax_rows": ("sampling", [c_void_p, c_int, c_void_p, c_int, c_int]),
+    "b200_beam_select": ("beam_select", [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         ctypes.c_longlong, c_int, c_int, c_int, c_int]),
+    "b200_copy_pages": ("cache_copy", [c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                       c_int, c_void_p]),
+    "b200_copy_slots": ("cache_copy", [c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, c_int, c_void_p, c_void_p,
+                                       c_int, c_void_p]),
+    "b200_attention_beams": ("attention_beams", [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                                 c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_int, c_int,
+                                                 c_int, c_int]),
     "b200_sample_rows": ("sampling", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_float, c_void_p]),
 }
 
@@ -1114,6 +1123,176 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, out: torch.Tensor,
                                    logits.shape[0], logits.shape[1], float(temperature), float(top_p),
                                    scratch.data_ptr() if scratch is not None else None, _stream()),
            "sample_rows")
+
+
+# --------------------------------------------------------------------------- beam search
+BEAM_MAX_KEEP = 256   # beam_select.cu
+
+
+def _here(*tensors: torch.Tensor) -> None:
+    """The tensors lie on the current device, on whose current stream a launch goes."""
+    _dev(*tensors)
+    for t in tensors:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def beam_select_takes(beams: int, keep: int) -> bool:
+    """Whether the selection takes that many beams of a request and that many continuations."""
+    return 1 <= beams <= 1024 and 1 <= keep <= BEAM_MAX_KEEP
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, out_scores: torch.Tensor, out_beams: torch.Tensor, out_tokens: torch.Tensor,
+                scratch: torch.Tensor | None = None) -> None:
+    """The best continuations of each request's beams, best first.  ``logits`` float32 [G * B, V] (rows may be apart); ``scores`` float32
+    [G, B]: the beams' log probabilities so far, -inf for a beam that does not count; results [G, n]: the n largest of scores[g, b] +
+    log softmax(logits[g B + b])[t] over beams and tokens, and their beams and tokens (int32).  Equal scores are ordered by beam, then by the
+    larger logit, then by token; sums are compared in 64 bits.  A token whose logit is -inf is never chosen, nor is anything of a row
+    that has no distribution (NaN, +inf or nothing but -inf); places left over hold -inf, -1, -1.  ``scratch``: uint8
+    workspace (allocated here when absent or too small)."""
+    _here(logits, scores, out_scores, out_beams, out_tokens, scratch)
+    if scores.dim() != 2 or out_scores.dim() != 2 or logits.dim() != 2:
+        raise KernelError("beam_select takes logits [G * B, V], scores [G, B] and results [G, n]")
+    (G, B), n = scores.shape, out_scores.shape[1]
+    assert logits.dtype == scores.dtype == out_scores.dtype == torch.float32 and out_beams.dtype == out_tokens.dtype == torch.int32
+    assert logits.shape[0] == G * B and logits.shape[1] >= 1 and (logits.stride(1) == 1 or logits.shape[1] == 1)
+    assert scores.is_contiguous() and all(t.is_contiguous() and tuple(t.shape) == (G, n) for t in (out_scores, out_beams, out_tokens))
+    if not beam_select_takes(B, n) or G * B > 65535:
+        raise KernelError(f"beam_select: {G} requests of {B} beams, {n} continuations each (at most 65,535 rows, 1,024 beams, "
+                          f"{BEAM_MAX_KEEP} continuations)")
+    if G == 0:
+        return
+    ld = logits.stride(0) if G * B > 1 else logits.shape[1]
+    need_fn = library("beam_select").b200_beam_select_scratch_bytes
+    need_fn.argtypes, need_fn.restype = [c_int, c_int, c_int], ctypes.c_longlong
+    need = int(need_fn(G * B, logits.shape[1], n))
+    if scratch is None or scratch.numel() < need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    assert scratch.dtype == torch.uint8 and scratch.is_contiguous() and scratch.data_ptr() % 16 == 0
+    _check(_fn("b200_beam_select")(logits.data_ptr(), ld, scores.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(),
+                                   out_tokens.data_ptr(), scratch.data_ptr(), scratch.numel(), G, B, logits.shape[1], n, _stream()),
+           "beam_select")
+
+
+def copy_groups(moves, n: int):
+    """Moves (source, destination, ...) by source, as the copy kernels take them: int32 arrays of the sources, of where each one's
+    destinations begin, and of the destinations, with the first move of each source.  Refuses numbers outside [0, n), a destination
+    that comes twice or is a source too."""
+    by_source: dict = {}
+    seen = set()
+    for m in moves:
+        s, d = int(m[0]), int(m[1])
+        if not (0 <= s < n and 0 <= d < n):
+            raise KernelError(f"a move from {s} to {d}: there are {n}")
+        if d in seen:
+            raise KernelError(f"{d} is the destination of two moves")
+        seen.add(d)
+        by_source.setdefault(s, []).append(m)
+    for s in by_source:
+        if s in seen:
+            raise KernelError(f"{s} is a source and a destination")
+    firsts = [0]
+    for group in by_source.values():
+        firsts.append(firsts[-1] + len(group))
+    ints = lambda xs: (c_int * max(1, len(xs)))(*xs)
+    return (ints(list(by_source)), ints(firsts), ints([int(m[1]) for group in by_source.values() for m in group]),
+            [group for group in by_source.values()])
+
+
+def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, moves) -> None:
+    """Copies the first positions of cache pages: for every (source, destination, positions) of ``moves`` positions 0 .. positions - 1 of
+    page ``source`` go to page ``destination``, in every entry and head; the destination's other positions stay.  Pools
+    [entries, pages, kv_heads, 64, head_dim] and [entries, pages, kv_heads, head_dim, 64], or of one entry without the first dimension.  A page
+    may be the source of several moves (read once; they must ask for as many positions), the destination of one, and not both."""
+    _here(k_pool, v_pool)
+    if k_pool.dim() == 4:
+        k_pool, v_pool = k_pool.unsqueeze(0), v_pool.unsqueeze(0)
+    E, P, H, T, D = k_pool.shape
+    assert k_pool.dtype == v_pool.dtype and T == PAGE_TOKENS and tuple(v_pool.shape) == (E, P, H, D, PAGE_TOKENS)
+    dtype_code(k_pool.dtype)
+    assert k_pool[0].is_contiguous() and v_pool[0].is_contiguous() and (E == 1 or k_pool.stride(0) == v_pool.stride(0))
+    sources, firsts, destinations, groups = copy_groups(moves, P)
+    positions = []
+    for group in groups:
+        n = int(group[0][2])
+        if not 0 <= n <= PAGE_TOKENS:
+            raise KernelError(f"{n} positions of a page of {PAGE_TOKENS}")
+        if any(int(m[2]) != n for m in group):
+            raise KernelError(f"page {group[0][0]} is copied with two numbers of positions")
+        positions.append(n)
+    if not groups:
+        return
+    counts = (c_int * len(positions))(*positions)
+    _check(_fn("b200_copy_pages")(k_pool.data_ptr(), v_pool.data_ptr(), k_pool.stride(0) if E > 1 else P * H * T * D, E, H, D,
+                                  k_pool.element_size(), ctypes.addressof(sources), ctypes.addressof(counts), ctypes.addressof(firsts),
+                                  len(groups), ctypes.addressof(destinations), _stream()), "copy_pages")
+
+
+def copy_slots(data: torch.Tensor, moves) -> None:
+    """Copies states of fixed size: for every (source, destination) of ``moves`` data[:, destination] = data[:, source].  ``data`` [entries,
+    slots, ...] of any type.  Sources and destinations as for ``copy_pages``."""
+    _here(data)
+    if data.dim() < 2:
+        raise KernelError("copy_slots takes data [entries, slots, ...]")
+    sources, firsts, destinations, groups = copy_groups(moves, data.shape[1])
+    if not groups or data.numel() == 0:
+        return
+    assert data[0, 0].is_contiguous()
+    size = data.element_size()
+    n_bytes = data[0, 0].numel() * size
+    # (a stride of 0, or one smaller than a state, would make two of them one)
+    assert data.shape[1] == 1 or data.stride(1) * size >= n_bytes
+    assert data.shape[0] == 1 or data.stride(0) * size >= n_bytes
+    _check(_fn("b200_copy_slots")(data.data_ptr(), data.stride(0) * size if data.shape[0] > 1 else 0, data.stride(1) * size, n_bytes,
+                                  data.shape[0], ctypes.addressof(sources), ctypes.addressof(firsts), len(groups),
+                                  ctypes.addressof(destinations), _stream()), "copy_slots")
+
+
+def attention_beams_supported(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
+    return dtype in _DTYPE_CODE and head_dim in (32, 64, 96, 128) and n_heads % n_kv_heads == 0 and n_heads // n_kv_heads <= 16
+
+
+def attention_beams_parts(n_groups: int, beams: int, n_heads: int, n_kv_heads: int, head_dim: int, capacity: int, dtype: torch.dtype,
+                          device) -> int:
+    """How many CTAs of a kv head share the pages of a step's groups: as many as the GPU holds at once, no more than there may be
+    pages (``capacity``: the longest sequence the launch must be right for)."""
+    per_sm = (3 if head_dim <= 64 else 2) if dtype == torch.bfloat16 else (2 if head_dim <= 64 else 1)
+    pages = (n_groups * -(-capacity // PAGE_TOKENS)) * -(-beams * (n_heads // n_kv_heads) // 64) + n_groups * beams
+    return max(1, min(per_sm * sm_count(torch.device(device)) // n_kv_heads, pages))
+
+
+def attention_decode_beams(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor,
+                           shared_pages: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, n_heads: int, n_kv_heads: int,
+                           head_dim: int, window: int, n_parts: int, scratch: torch.Tensor | None = None) -> None:
+    """``attention_decode`` for sequences in groups of equal size that share their first pages (the beams of a request): group g is
+    sequences g B .. (g + 1) B - 1, and the first shared_pages[g] entries of their rows of the page table are the same (int32 [groups]; pages
+    that are not full for all of the group's sequences count as each one's own).  ``n_parts``: see ``attention_beams_parts``."""
+    _here(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, scratch)
+    n_seqs, n_groups = out.shape[0], shared_pages.numel()
+    if not attention_beams_supported(q.dtype, n_heads, n_kv_heads, head_dim):
+        raise KernelError(f"attention_decode_beams: {n_heads} heads on {n_kv_heads} of {head_dim} in {q.dtype}")
+    if n_groups == 0 or n_seqs % n_groups:
+        raise KernelError(f"{n_seqs} sequences do not make {n_groups} equal groups")
+    assert q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and out.is_contiguous() and out.shape[1] == n_heads * head_dim
+    assert q.stride(-1) == 1 and q_row_stride >= n_heads * head_dim
+    for t in (kv_lens, page_table, shared_pages):
+        assert t.dtype == torch.int32 and t.is_contiguous()
+    assert kv_lens.numel() == n_seqs and page_table.shape[0] == n_seqs
+    assert tuple(k_pool.shape[1:]) == (n_kv_heads, PAGE_TOKENS, head_dim) and k_pool.is_contiguous()
+    assert tuple(v_pool.shape[1:]) == (n_kv_heads, head_dim, PAGE_TOKENS) and v_pool.is_contiguous()
+    if n_seqs == 0:
+        return
+    B = n_seqs // n_groups
+    need_fn = library("attention_beams").b200_attention_beams_scratch_floats
+    need_fn.argtypes, need_fn.restype = [c_int] * 6, ctypes.c_longlong
+    need = int(need_fn(n_groups, B, n_heads, n_kv_heads, head_dim, n_parts))
+    if scratch is None or scratch.numel() < need:
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+    assert scratch.dtype == torch.float32 and scratch.is_contiguous()
+    _check(_fn("b200_attention_beams")(
+        q.data_ptr(), q_row_stride, out.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), page_table.shape[1], shared_pages.data_ptr(),
+        k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), n_groups, B, n_heads, n_kv_heads, head_dim, int(window),
+        n_parts, dtype_code(q.dtype), _stream()), "attention_decode_beams")
 
 
 # --------------------------------------------------------------------------- several residual streams
