@@ -5,8 +5,8 @@
 // ordered by total, ties by the lower beam, then the larger logit, then the lower token.  Within a row the order of the totals
 // is that of the logits, so each row's own best `keep` are found among the logits, without its lse; only those meet the
 // other beams' on one scale.  Two launches:
-//   beam_rows   a CTA per (chunk of a row, row): the chunk is read once, into registers, and leaves its maximum, its sum of
-//               exponentials and its best `keep` logits in order;
+//   beam_rows   a CTA per (chunk of a row, row): the chunk is read once, by warps that work by themselves, and leaves a sum of
+//               exponentials with what they are relative to and its best `keep` logits in order;
 //   beam_merge  a CTA per request: the rows' lse from their chunks' maxima and sums, the totals of what the chunks left, and
 //               the best of those.
 // Exponentials are taken in 32 bits and added in 32 bits over a thread's sixteen and a warp's lanes, from there on in 64: a
@@ -23,10 +23,11 @@ namespace b200 {
 
 constexpr int kBeamThreads = 256;                       // of beam_rows
 constexpr int kBeamWarps = kBeamThreads / 32;
-constexpr int kBeamEach = 16;                           // logits of a thread
-constexpr int kBeamChunk = kBeamThreads * kBeamEach;    // logits of a CTA
-constexpr int kBeamList = 512;                          // candidates that are ordered by counting
+constexpr int kBeamEach = 16;                           // logits of a thread at a time
+constexpr int kBeamTile = kBeamThreads * kBeamEach;
 constexpr int kBeamMaxKeep = 256;
+constexpr int kBeamLimit = 512;                         // candidates from which a CTA's list is cut down
+constexpr int kBeamList = kBeamLimit + kBeamTile;       // most that it holds
 constexpr int kMergeThreads = 512;
 constexpr int kMergeList = 1024;
 
@@ -57,142 +58,181 @@ __device__ __forceinline__ float from_rising_bits(unsigned r) {
 }
 constexpr unsigned kRisingMinusInf = 0x007fffffu;
 
-__global__ void __launch_bounds__(kBeamThreads)
-beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __restrict__ scores, int vocab, int keep, int vec,
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+typedef unsigned long long u64;
+// A candidate as one number: a larger logit, of equal ones a lower token, is the larger number.
+__device__ __forceinline__ u64 beam_key(float x, int token) { return ((u64)rising_bits(x) << 32) | (0xffffffffu - (unsigned)token); }
+
+struct RowsShared {
+    u64 list[kBeamList];                // 36 KB
+    int n;
+    unsigned warp_key[kBeamWarps];
+    float ref[kBeamWarps];
+    double sum[kBeamWarps];
+    int count[2][kBeamWarps];
+};
+
+// Cuts the CTA's list (more than `keep` candidates) down to its best, at least `keep` and at most a quarter more.  What they reach is
+// searched for bit by bit, candidates of equal logits by their tokens.  Returns its upper half.  All threads call it, behind a barrier.
+__device__ __forceinline__ unsigned cut_down(RowsShared& sh, int keep) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = sh.n;
+    int round = 0;
+    auto total = [&](int mine) {
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        round ^= 1;                     // (two sets of counts in turn: one barrier a count)
+        if (lane == 0) sh.count[round][warp] = mine;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kBeamWarps; ++w) all += sh.count[round][w];
+        return all;
+    };
+    u64 least = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const u64 t = least | (1ull << bit);
+        int mine = 0;
+        for (int i = tid; i < n; i += kBeamThreads) mine += sh.list[i] >= t ? 1 : 0;
+        mine = total(mine);
+        if (mine >= keep) {
+            least = t;
+            if (mine <= keep + keep / 4) break;
+        }
+    }
+    // in place, a stretch of 256 after the other: nothing goes behind where it was
+    int kept = 0;
+    for (int i0 = 0; i0 < n; i0 += kBeamThreads) {
+        const u64 key = i0 + tid < n ? sh.list[i0 + tid] : 0ull;
+        const bool in = key >= least && key != 0ull;
+        const unsigned mask = __ballot_sync(0xffffffffu, in);
+        round ^= 1;
+        if (lane == 0) sh.count[round][warp] = __popc(mask);
+        __syncthreads();
+        int at = kept;
+#pragma unroll
+        for (int w = 0; w < kBeamWarps; ++w) {
+            if (w < warp) at += sh.count[round][w];
+            kept += sh.count[round][w];
+        }
+        if (in) sh.list[at + __popc(mask & ((1u << lane) - 1u))] = key;
+    }
+    if (tid == 0) sh.n = kept;
+    __syncthreads();
+    return (unsigned)(least >> 32);
+}
+
+__global__ void __launch_bounds__(kBeamThreads, 4)
+beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __restrict__ scores, int vocab, int keep, int vec, int tiles,
                  BeamScratch out) {
-    __shared__ float warp_max_s[kBeamWarps], warp_sum_s[kBeamWarps];
-    __shared__ unsigned warp_key_s[kBeamWarps];
-    __shared__ float list_x[kBeamList];
-    __shared__ int list_t[kBeamList];
-    __shared__ int list_n;
-    __shared__ unsigned long long warp_best_s[kBeamWarps];
+    __shared__ RowsShared sh;
+    const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) sh.n = 0;
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float score = scores[row];
     if (!(fabsf(score) < INFINITY)) return;     // (the merge does not look at this row either)
     const size_t piece = (size_t)row * gridDim.x + blockIdx.x;
-    const int base = blockIdx.x * kBeamChunk, n = min(kBeamChunk, vocab - base);
-    const float* x0 = logits + (size_t)row * ld + base;
+    const int first = blockIdx.x * tiles * kBeamTile, end = min(vocab, first + tiles * kBeamTile);
+    const float* x_row = logits + (size_t)row * ld;
 
-    float x[kBeamEach];
-    auto place = [&](int e) {       // of a thread's element e in the chunk
-        return vec ? ((e >> 2) * kBeamThreads + tid) * 4 + (e & 3) : e * kBeamThreads + tid;
-    };
-    if (vec) {
+    auto place = [&](int e) { return vec ? ((e >> 2) * kBeamThreads + tid) * 4 + (e & 3) : e * kBeamThreads + tid; };    // in a tile
+    auto load = [&](float (&x)[kBeamEach], int base) {
+        const int n = end - base;
+        const float* x0 = x_row + base;
+        if (vec && n >= kBeamTile) {
 #pragma unroll
-        for (int u = 0; u < kBeamEach / 4; ++u) {
-            const int at = (u * kBeamThreads + tid) * 4;
-            if (at + 4 <= n) {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(x0 + at));
+            for (int u = 0; u < kBeamEach / 4; ++u) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(x0) + u * kBeamThreads + tid);
                 x[4 * u] = v.x; x[4 * u + 1] = v.y; x[4 * u + 2] = v.z; x[4 * u + 3] = v.w;
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[4 * u + c] = at + c < n ? x0[at + c] : -INFINITY;
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kBeamEach; ++e) x[e] = place(e) < n ? __ldg(x0 + place(e)) : -INFINITY;
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < kBeamEach; ++e) x[e] = place(e) < n ? x0[place(e)] : -INFINITY;
-    }
-    float mine = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < kBeamEach; ++e) { x[e] += 0.f; mine = fmaxf(mine, x[e]); }     // (-0 counts as 0)
-    if (tid == 0) list_n = 0;
-
-    // The warp's maximum and sum, and the j-th largest of its lanes' maxima: the warps' smallest such number is one that at
-    // least warps * j >= keep logits reach, and few more than that do.
+    };
     const int j = (keep + kBeamWarps - 1) / kBeamWarps;
-    unsigned key = rising_bits(mine), threshold = 0;
-    float m = -INFINITY;
-    if (j <= 32) {
-        for (int i = 0; i < j; ++i) {
-            threshold = __reduce_max_sync(0xffffffffu, key);
-            if (i == 0) m = from_rising_bits(threshold);
-            const unsigned at = __ballot_sync(0xffffffffu, key == threshold);
-            if (lane == __ffs(at) - 1) key = 0;
+    float border = 0.f;         // what candidates reach
+    float ref = -INFINITY;      // the thread's exponentials are relative to it
+    double total = 0.0;
+    float x[kBeamEach], ahead[kBeamEach];
+    load(ahead, first);
+    for (int base = first; base < end; base += kBeamTile) {
+#pragma unroll
+        for (int e = 0; e < kBeamEach; ++e) x[e] = ahead[e];
+        if (base + kBeamTile < end) load(ahead, base + kBeamTile);
+        float mine = x[0];
+#pragma unroll
+        for (int e = 1; e < kBeamEach; ++e) mine = fmaxf(mine, x[e]);
+
+        if (base == first) {
+            // The j-th largest of the warp's lanes' maxima: the least of the warps' such numbers is one that at least warps * j >= keep
+            // logits reach, and few more than that do.
+            unsigned key = isnan(mine) ? 0u : rising_bits(mine), nth = __reduce_max_sync(0xffffffffu, key);
+            ref = nth ? from_rising_bits(nth) : -INFINITY;
+            for (int i = 1; i < j; ++i) {
+                const unsigned at = __ballot_sync(0xffffffffu, key == nth);
+                if (lane == __ffs(at) - 1) key = 0;
+                nth = __reduce_max_sync(0xffffffffu, key);
+            }
+            if (lane == 0) sh.warp_key[warp] = nth;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kBeamWarps; ++w) nth = min(nth, sh.warp_key[w]);
+            border = from_rising_bits(max(nth, kRisingMinusInf + 1u));       // -inf is no candidate
         }
-    }
-    float sum = 0.f;
-    if (m > -INFINITY) {
+        if (mine > ref + 16.f) {        // (relative to the maximum of the warp's first logits until that is exceeded by far)
+            if (ref > -INFINITY) total *= (double)expf(ref - mine);
+            ref = mine;
+        }
+        const float zero = ref == -INFINITY ? 0.f : ref;     // (nothing but -inf so far, or NaN, which has to show)
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < kBeamEach; ++e) sum += expf(x[e] - m);
-    } else {        // nothing but -inf, or NaN: which has to show
+        for (int e = 0; e < kBeamEach; ++e) sum[e & 1] += exp2_fast((x[e] - zero) * 1.4426950408889634f);
+        total += (double)(sum[0] + sum[1]);
+
+        if (mine >= border) {
 #pragma unroll
-        for (int e = 0; e < kBeamEach; ++e) if (isnan(x[e])) sum = x[e];
+            for (int e = 0; e < kBeamEach; ++e)
+                if (x[e] >= border) sh.list[atomicAdd(&sh.n, 1)] = beam_key(x[e] + 0.f, base + place(e));        // (-0 counts as 0)
+        }
+        __syncthreads();
+        if (sh.n > kBeamLimit) border = fmaxf(border, from_rising_bits(cut_down(sh, keep)));
     }
-    sum = warp_sum(sum);
-    if (lane == 0) {
-        warp_max_s[warp] = m;
-        warp_sum_s[warp] = sum;
-        warp_key_s[warp] = threshold;
+    {
+        const float r = warp_max(ref);
+        if (ref < r && ref > -INFINITY) total *= exp((double)ref - (double)r);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (lane == 0) { sh.ref[warp] = r; sh.sum[warp] = total; }
     }
     __syncthreads();
-    unsigned least = 0xffffffffu;
+    if (sh.n > keep + 32) cut_down(sh, keep);
+    if (warp == 0) {
+        const float w = lane < kBeamWarps ? sh.ref[lane] : -INFINITY, r = warp_max(w);
+        double t = lane < kBeamWarps ? sh.sum[lane] : 0.0;
+        if (w < r && w > -INFINITY) t *= exp((double)w - (double)r);
 #pragma unroll
-    for (int w = 0; w < kBeamWarps; ++w) least = min(least, warp_key_s[w]);
-    least = max(least, kRisingMinusInf + 1u);           // -inf is no candidate
-    if (tid == 0) {
-        float top = -INFINITY;
-        for (int w = 0; w < kBeamWarps; ++w) top = fmaxf(top, warp_max_s[w]);
-        double total = 0.0;
-        for (int w = 0; w < kBeamWarps; ++w) {
-            const double s = (double)warp_sum_s[w];
-            total += warp_max_s[w] > -INFINITY ? s * exp((double)warp_max_s[w] - (double)top) : s;
-        }
-        out.maxima[piece] = top;
-        out.sums[piece] = total;
+        for (int o = kBeamWarps / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (lane == 0) { out.maxima[piece] = r; out.sums[piece] = t; }
     }
-    const float border = from_rising_bits(least);
-#pragma unroll
-    for (int e = 0; e < kBeamEach; ++e) {
-        if (x[e] >= border) {
-            const int i = atomicAdd(&list_n, 1);
-            if (i < kBeamList) { list_x[i] = x[e]; list_t[i] = base + place(e); }
-        }
-    }
-    __syncthreads();
+    // in order: every candidate's place is the number of those before it
+    const int found = sh.n;
     float* to_x = out.logits + piece * keep;
     int* to_t = out.tokens + piece * keep;
-    const int found = list_n;
-    if (found <= kBeamList) {
-        // the list's order does not matter: every candidate's place is the number of those before it
-        for (int i = tid; i < found; i += kBeamThreads) {
-            const float v = list_x[i];
-            const int t = list_t[i];
-            int before = 0;
-            for (int k = 0; k < found; ++k) before += (list_x[k] > v || (list_x[k] == v && list_t[k] < t)) ? 1 : 0;
-            if (before < keep) { to_x[before] = v; to_t[before] = t; }
-        }
-        for (int i = found + tid; i < keep; i += kBeamThreads) to_t[i] = -1;
-        return;
-    }
-    // Many logits reach the border (a chunk that is masked for the most part, or holds equal numbers): one after the other.
-    for (int r = 0; r < keep; ++r) {
-        unsigned long long best = 0;    // the rising bits, then the lower place
-#pragma unroll
-        for (int e = 0; e < kBeamEach; ++e) {
-            const unsigned b = rising_bits(x[e]);
-            if (x[e] > -INFINITY) best = max(best, ((unsigned long long)b << 32) | (unsigned)(0xffffffffu - place(e)));
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if (lane == 0) warp_best_s[warp] = best;
-        __syncthreads();
-        best = warp_best_s[0];
-#pragma unroll
-        for (int w = 1; w < kBeamWarps; ++w) best = max(best, warp_best_s[w]);
-        __syncthreads();
-        const int at = (int)(0xffffffffu - (unsigned)best);
-        if (tid == 0) {
-            to_x[r] = best ? from_rising_bits((unsigned)(best >> 32)) : -INFINITY;
-            to_t[r] = best ? base + at : -1;
-        }
-        if (best) {
-#pragma unroll
-            for (int e = 0; e < kBeamEach; ++e) if (place(e) == at) x[e] = -INFINITY;
+    for (int i = tid; i < found; i += kBeamThreads) {
+        const u64 key = sh.list[i];
+        int before = 0;
+        for (int k = 0; k < found; ++k) before += sh.list[k] > key ? 1 : 0;
+        if (before < keep) {
+            to_x[before] = from_rising_bits((unsigned)(key >> 32));
+            to_t[before] = (int)(0xffffffffu - (unsigned)key);
         }
     }
+    for (int i = found + tid; i < keep; i += kBeamThreads) to_t[i] = -1;
 }
 
 struct Candidate {
@@ -209,19 +249,26 @@ __device__ __forceinline__ bool goes_before(const Candidate& a, const Candidate&
     return a.token < b.token;
 }
 
+constexpr int kMergeKeys = 4096;
+struct MergeShared {
+    u64 keys[kMergeKeys];               // candidates of the lists that may hold some of the best: total rounded down to 32 bits, number
+    double total[kMergeList];
+    float logit[kMergeList];
+    int beam[kMergeList], token[kMergeList];
+    int active[kMergeList];             // those lists
+    Candidate warp_best[kMergeThreads / 32];
+    int n_keys, n_active, n;
+};
+
 __global__ void __launch_bounds__(kMergeThreads)
 beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int keep, BeamScratch in, float* __restrict__ out_scores,
                   int* __restrict__ out_beams, int* __restrict__ out_tokens) {
-    __shared__ double list_total[kMergeList];
-    __shared__ float list_logit[kMergeList];
-    __shared__ int list_beam[kMergeList], list_token[kMergeList];
-    __shared__ int list_n;
-    __shared__ unsigned warp_key_s[kMergeThreads / 32];
-    __shared__ Candidate warp_best_s[kMergeThreads / 32];
-    extern __shared__ double lse_s[];       // [beams]; NaN: the row gives none
+    extern __shared__ __align__(16) unsigned char merge_smem[];
+    MergeShared& sh = *reinterpret_cast<MergeShared*>(merge_smem);
+    double* lse_s = reinterpret_cast<double*>(merge_smem + sizeof(MergeShared));        // [beams]; NaN: the row gives none
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = kMergeThreads / 32;
-    if (tid == 0) list_n = 0;
+    if (tid == 0) sh.n = sh.n_active = sh.n_keys = 0;
     pdl_launch_dependents();
     pdl_wait();
     for (int b = warp; b < beams; b += kWarps) {
@@ -263,43 +310,95 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         return c;
     };
 
-    // As in beam_rows: of every warp's lists the j-th best head, rounded down to 32 bits; at least `keep` candidates reach the least of them.
-    const int used_warps = min(kWarps, (lists + 31) / 32), j = (keep + used_warps - 1) / used_warps;
-    unsigned key = 0, threshold = 0;
+    // A number that at least `keep` candidates reach (rounded down to 32 bits) and not many more: where there are lists enough, one that `keep` of the
+    // threads' best reach; where there are few, one that so many of their (depth + 1)-th best reach that it comes to as much.  None: all candidates.
+    bool head = false;
+    for (int l = tid; l < lists; l += kMergeThreads) head = head || candidate(l, 0).token >= 0;
+    const int n_heads = __syncthreads_count(head);
+    const int depth = n_heads >= keep || n_heads == 0 ? 0 : (2 * keep + n_heads - 1) / n_heads - 1, need = (keep + depth) / (depth + 1);
+    unsigned key = 0;
     for (int l = tid; l < lists; l += kMergeThreads) {
-        const Candidate c = candidate(l, 0);
+        const Candidate c = candidate(l, depth);
         if (c.token >= 0) key = max(key, rising_bits(__double2float_rd(c.total)));
     }
-    if (j <= 32) {
-        for (int i = 0; i < j; ++i) {
-            threshold = __reduce_max_sync(0xffffffffu, key);
-            const unsigned at = __ballot_sync(0xffffffffu, key == threshold);
-            if (lane == __ffs(at) - 1) key = 0;
+    unsigned least = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned t = least | (1u << bit);
+        const int n = __syncthreads_count(key >= t);
+        if (n >= need) least = t;
+        if (n >= need && n <= need + need / 4) break;
+    }
+    least = max(least, 1u);
+    // the lists with a candidate that reaches it, a thread each; then of those, a warp each, all that reach it
+    for (int l = tid; l < lists; l += kMergeThreads) {
+        const Candidate c = candidate(l, 0);
+        if (c.token >= 0 && rising_bits(__double2float_rd(c.total)) >= least) {
+            const int i = atomicAdd(&sh.n_active, 1);
+            if (i < kMergeList) sh.active[i] = l;
         }
     }
-    if (lane == 0) warp_key_s[warp] = threshold;
     __syncthreads();
-    unsigned least = 0xffffffffu;
-    for (int w = 0; w < used_warps; ++w) least = min(least, warp_key_s[w]);
-    for (int l = tid; l < lists; l += kMergeThreads) {
-        for (int k = 0; k < keep; ++k) {
-            const Candidate c = candidate(l, k);
-            if (c.token < 0 || rising_bits(__double2float_rd(c.total)) < least) break;
-            const int i = atomicAdd(&list_n, 1);
-            if (i < kMergeList) { list_total[i] = c.total; list_logit[i] = c.logit; list_beam[i] = c.beam; list_token[i] = c.token; }
+    const int n_active = sh.n_active;
+    for (int a = warp; a < min(n_active, kMergeList); a += kWarps) {
+        for (int k0 = 0; k0 < keep; k0 += 32) {
+            const Candidate c = candidate(sh.active[a], k0 + lane);
+            const unsigned b = rising_bits(__double2float_rd(c.total));
+            const bool in = c.token >= 0 && b >= least;
+            if (in) {
+                const int i = atomicAdd(&sh.n_keys, 1);
+                if (i < kMergeKeys) sh.keys[i] = ((u64)b << 32) | (unsigned)(sh.active[a] * keep + k0 + lane);
+            }
+            if (!__any_sync(0xffffffffu, in)) break;
+        }
+    }
+    __syncthreads();
+    const int n_keys = sh.n_keys;
+    if (n_active <= kMergeList && n_keys <= kMergeKeys) {
+        constexpr int kEach = kMergeKeys / kMergeThreads;
+        u64 mine[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) mine[u] = tid + u * kMergeThreads < n_keys ? sh.keys[tid + u * kMergeThreads] : 0ull;
+        if (n_keys > keep + keep / 4) {     // the same search over all of these
+            least = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned t = least | (1u << bit);
+                int n = 0;
+#pragma unroll
+                for (int u = 0; u < kEach; ++u) n += (unsigned)(mine[u] >> 32) >= t ? 1 : 0;
+                n = __reduce_add_sync(0xffffffffu, n);
+                __shared__ int count[2][kWarps];
+                if (lane == 0) count[bit & 1][warp] = n;
+                __syncthreads();
+                n = 0;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) n += count[bit & 1][w];
+                if (n >= keep) {
+                    least = t;
+                    if (n <= keep + keep / 4) break;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            if ((unsigned)(mine[u] >> 32) >= max(least, 1u)) {
+                const unsigned number = (unsigned)mine[u];
+                const Candidate c = candidate(number / keep, number % keep);
+                const int i = atomicAdd(&sh.n, 1);
+                if (i < kMergeList) { sh.total[i] = c.total; sh.logit[i] = c.logit; sh.beam[i] = c.beam; sh.token[i] = c.token; }
+            }
         }
     }
     __syncthreads();
     const size_t to = (size_t)g * keep;
-    const int found = list_n;
+    const int found = n_active <= kMergeList && n_keys <= kMergeKeys ? sh.n : kMergeList + 1;
     if (found <= kMergeList) {
         for (int i = tid; i < found; i += kMergeThreads) {
-            const Candidate c{list_total[i], list_logit[i], list_beam[i], list_token[i]};
+            const Candidate c{sh.total[i], sh.logit[i], sh.beam[i], sh.token[i]};
             int before = 0;
             for (int k = 0; k < found; ++k) {
-                const double o = list_total[k];
+                const double o = sh.total[k];
                 if (o > c.total) ++before;
-                else if (o == c.total) before += goes_before(Candidate{o, list_logit[k], list_beam[k], list_token[k]}, c) ? 1 : 0;
+                else if (o == c.total) before += goes_before(Candidate{o, sh.logit[k], sh.beam[k], sh.token[k]}, c) ? 1 : 0;
             }
             if (before < keep) {
                 out_scores[to + before] = (float)c.total;
@@ -337,10 +436,10 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
             c.token = __shfl_xor_sync(0xffffffffu, best.token, o);
             if (goes_before(c, best)) best = c;
         }
-        if (lane == 0) warp_best_s[warp] = best;
+        if (lane == 0) sh.warp_best[warp] = best;
         __syncthreads();
-        best = warp_best_s[0];
-        for (int w = 1; w < kWarps; ++w) if (goes_before(warp_best_s[w], best)) best = warp_best_s[w];
+        best = sh.warp_best[0];
+        for (int w = 1; w < kWarps; ++w) if (goes_before(sh.warp_best[w], best)) best = sh.warp_best[w];
         __syncthreads();
         last = best;
         if (tid == 0) {
@@ -361,10 +460,19 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
 
 }  // namespace b200
 
+namespace b200 {
+// Tiles of a CTA: so many that all rows' CTAs are on the GPU at once, four an SM; the tiles behind the first meet a border that few of
+// their logits reach, and the merge has fewer lists.  Rows beyond that are a CTA each.
+static int tiles_of(long long rows, int vocab) {
+    const long long tiles = (vocab + kBeamTile - 1) / kBeamTile, ctas = 4ll * device_sm_count() / rows;
+    return (int)(ctas < 1 ? tiles : (tiles + ctas - 1) / ctas);
+}
+}  // namespace b200
+
 // Bytes of scratch (16-byte aligned) that a call needs.
 extern "C" long long b200_beam_select_scratch_bytes(int n_rows, int vocab, int keep) {
-    const long long pieces = (long long)n_rows * ((vocab + b200::kBeamChunk - 1) / b200::kBeamChunk);
-    return pieces * (12 + 8ll * keep);
+    const int chunk = b200::tiles_of(n_rows, vocab) * b200::kBeamTile;
+    return (long long)n_rows * ((vocab + chunk - 1) / chunk) * (12 + 8ll * keep);
 }
 
 // logits: [n_groups * beams] rows of `vocab` floats, `ld` apart; scores: [n_groups, beams]; outputs: [n_groups, keep].
@@ -374,14 +482,23 @@ extern "C" int b200_beam_select(const float* logits, long long ld, const float* 
     if (n_groups <= 0) return 0;
     if (beams < 1 || vocab < 1 || keep < 1 || ld < vocab) return kErrBadArgument;
     if (keep > kBeamMaxKeep || beams > 1024 || (long long)n_groups * beams > 65535) return kErrUnsupportedSize;
-    const int chunks = (vocab + kBeamChunk - 1) / kBeamChunk;
     const long long rows = (long long)n_groups * beams;
+    const int tiles = tiles_of(rows, vocab), chunks = (vocab + tiles * kBeamTile - 1) / (tiles * kBeamTile);
     if (scratch_bytes < b200_beam_select_scratch_bytes((int)rows, vocab, keep)) return 10003;
     const BeamScratch s = beam_scratch(scratch, rows * chunks, keep);
     const int vec = ((uintptr_t)logits & 15) == 0 && (ld & 3) == 0;
+    const size_t merge_bytes = sizeof(MergeShared) + sizeof(double) * beams;
+    static bool configured[64] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
+    if (!configured[device]) {
+        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(MergeShared) + 8 * 1024));
+        if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
+        configured[device] = true;
+    }
     const int st = launch_pdl(beam_rows_kernel, dim3(chunks, (unsigned)rows), dim3(kBeamThreads), 0, stream, logits, ld, scores, vocab, keep,
-                              vec, s);
+                              vec, tiles, s);
     if (st != 0) return st;
-    return launch_pdl(beam_merge_kernel, dim3(n_groups), dim3(kMergeThreads), sizeof(double) * beams, stream, scores, beams, chunks, keep, s,
+    return launch_pdl(beam_merge_kernel, dim3(n_groups), dim3(kMergeThreads), merge_bytes, stream, scores, beams, chunks, keep, s,
                       out_scores, out_beams, out_tokens);
 }
