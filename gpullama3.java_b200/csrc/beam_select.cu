@@ -1,6 +1,6 @@
 // A beam search's selection: of every request's beams and the whole vocabulary, the `keep` best continuations.
 //
-//   total[g, b, t] = scores[g, b] + (x[g, b, t] - lse[g, b]),   lse = m + log sum_t exp(x_t - m),   m = max_t x_t
+//   total[g, b, t] = scores[g, b] + (x[g, b, t] - m) - log sum_t exp(x_t - m),   m = max_t x_t
 //
 // ordered by total, ties by the lower beam, then the larger logit, then the lower token.  Within a row the order of the totals
 // is that of the logits, so each row's own best `keep` are found among the logits, without its lse; only those meet the
@@ -26,25 +26,25 @@ constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamEach = 16;                           // logits of a thread at a time
 constexpr int kBeamTile = kBeamThreads * kBeamEach;
 constexpr int kBeamMaxKeep = 256;
-constexpr int kBeamLimit = 512;                         // candidates from which a CTA's list is cut down
+constexpr int kBeamLimit = 768;                         // most candidates of a list that is not cut down (3 keep)
 constexpr int kBeamList = kBeamLimit + kBeamTile;       // most that it holds
 constexpr int kMergeThreads = 512;
 constexpr int kMergeList = 1024;
 
-// What a chunk leaves: [row][chunk] maximum (float) and sum (double), then [row][chunk][keep] logit and token, the best first, tokens of -1
-// behind the last.
+typedef unsigned long long u64;
+
+// What a chunk leaves: [row][chunk] a sum of exponentials and what they are relative to, [row][chunk][keep] candidates, the best first, zeros behind
+// the last.
 struct BeamScratch {
     double* sums;
+    u64* candidates;
     float* maxima;
-    float* logits;
-    int* tokens;
 };
 __host__ __device__ inline BeamScratch beam_scratch(void* base, long long pieces, int keep) {
     BeamScratch s;
     s.sums = (double*)base;
-    s.maxima = (float*)(s.sums + pieces);
-    s.logits = s.maxima + pieces;
-    s.tokens = (int*)(s.logits + pieces * keep);
+    s.candidates = (u64*)(s.sums + pieces);
+    s.maxima = (float*)(s.candidates + pieces * keep);
     return s;
 }
 
@@ -64,17 +64,19 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-typedef unsigned long long u64;
 // A candidate as one number: a larger logit, of equal ones a lower token, is the larger number.
 __device__ __forceinline__ u64 beam_key(float x, int token) { return ((u64)rising_bits(x) << 32) | (0xffffffffu - (unsigned)token); }
+__device__ __forceinline__ float key_logit(u64 key) { return from_rising_bits((unsigned)(key >> 32)); }
+__device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (unsigned)key); }
 
 struct RowsShared {
     u64 list[kBeamList];                // 36 KB
     int n;
-    unsigned warp_key[kBeamWarps];
+    unsigned best[kBeamThreads];        // the threads' maxima of the first tile
     float ref[kBeamWarps];
     double sum[kBeamWarps];
     int count[2][kBeamWarps];
+    unsigned high[kBeamWarps], low[kBeamWarps];
 };
 
 // Cuts the CTA's list (more than `keep` candidates) down to its best, at least `keep` and at most a quarter more.  What they reach is
@@ -92,8 +94,21 @@ __device__ __forceinline__ unsigned cut_down(RowsShared& sh, int keep) {
         for (int w = 0; w < kBeamWarps; ++w) all += sh.count[round][w];
         return all;
     };
-    u64 least = 0;
-    for (int bit = 63; bit >= 0; --bit) {
+    // (the bits that all candidates have in common are not searched)
+    unsigned high = 0, low = 0xffffffffu;
+    for (int i = tid; i < n; i += kBeamThreads) {
+        high = max(high, (unsigned)(sh.list[i] >> 32));
+        low = min(low, (unsigned)(sh.list[i] >> 32));
+    }
+    high = __reduce_max_sync(0xffffffffu, high);
+    low = __reduce_min_sync(0xffffffffu, low);
+    if (lane == 0) { sh.high[warp] = high; sh.low[warp] = low; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBeamWarps; ++w) { high = max(high, sh.high[w]); low = min(low, sh.low[w]); }
+    const int differing = 32 - __clz(high ^ low);
+    u64 least = differing == 32 ? 0ull : ((u64)high << 32) >> (32 + differing) << (32 + differing);
+    for (int bit = 31 + differing; bit >= 0; --bit) {
         const u64 t = least | (1ull << bit);
         int mine = 0;
         for (int i = tid; i < n; i += kBeamThreads) mine += sh.list[i] >= t ? 1 : 0;
@@ -154,7 +169,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
             for (int e = 0; e < kBeamEach; ++e) x[e] = place(e) < n ? __ldg(x0 + place(e)) : -INFINITY;
         }
     };
-    const int j = (keep + kBeamWarps - 1) / kBeamWarps;
+    const int limit = max(128, 3 * keep);
     float border = 0.f;         // what candidates reach
     float ref = -INFINITY;      // the thread's exponentials are relative to it
     double total = 0.0;
@@ -169,20 +184,27 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
         for (int e = 1; e < kBeamEach; ++e) mine = fmaxf(mine, x[e]);
 
         if (base == first) {
-            // The j-th largest of the warp's lanes' maxima: the least of the warps' such numbers is one that at least warps * j >= keep
-            // logits reach, and few more than that do.
-            unsigned key = isnan(mine) ? 0u : rising_bits(mine), nth = __reduce_max_sync(0xffffffffu, key);
-            ref = nth ? from_rising_bits(nth) : -INFINITY;
-            for (int i = 1; i < j; ++i) {
-                const unsigned at = __ballot_sync(0xffffffffu, key == nth);
-                if (lane == __ffs(at) - 1) key = 0;
-                nth = __reduce_max_sync(0xffffffffu, key);
-            }
-            if (lane == 0) sh.warp_key[warp] = nth;
+            // What about the keep-th largest of the threads' maxima reach, at least `keep` logits do, and few more.
+            const unsigned key = isnan(mine) ? 0u : rising_bits(mine);
+            sh.best[tid] = key;
+            const unsigned top = __reduce_max_sync(0xffffffffu, key);
+            ref = top ? from_rising_bits(top) : -INFINITY;
             __syncthreads();
+            unsigned best[kBeamThreads / 32], least = 0;
 #pragma unroll
-            for (int w = 0; w < kBeamWarps; ++w) nth = min(nth, sh.warp_key[w]);
-            border = from_rising_bits(max(nth, kRisingMinusInf + 1u));       // -inf is no candidate
+            for (int u = 0; u < kBeamThreads / 32; ++u) best[u] = sh.best[u * 32 + lane];
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned t = least | (1u << bit);
+                int n = 0;
+#pragma unroll
+                for (int u = 0; u < kBeamThreads / 32; ++u) n += best[u] >= t ? 1 : 0;
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (n >= keep) {
+                    least = t;
+                    if (n <= keep + keep / 4) break;
+                }
+            }
+            border = from_rising_bits(max(least, kRisingMinusInf + 1u));     // -inf is no candidate
         }
         if (mine > ref + 16.f) {        // (relative to the maximum of the warp's first logits until that is exceeded by far)
             if (ref > -INFINITY) total *= (double)expf(ref - mine);
@@ -195,12 +217,20 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
         total += (double)(sum[0] + sum[1]);
 
         if (mine >= border) {
+            unsigned hits = 0;
 #pragma unroll
-            for (int e = 0; e < kBeamEach; ++e)
-                if (x[e] >= border) sh.list[atomicAdd(&sh.n, 1)] = beam_key(x[e] + 0.f, base + place(e));        // (-0 counts as 0)
+            for (int e = 0; e < kBeamEach; ++e) hits |= x[e] >= border ? 1u << e : 0u;
+            int at = atomicAdd(&sh.n, __popc(hits));
+            for (; hits; hits &= hits - 1) {
+                const int e = __ffs(hits) - 1;
+                float v = x[0];
+#pragma unroll
+                for (int k = 1; k < kBeamEach; ++k) v = e == k ? x[k] : v;
+                sh.list[at++] = beam_key(v + 0.f, base + place(e));      // (-0 counts as 0)
+            }
         }
         __syncthreads();
-        if (sh.n > kBeamLimit) border = fmaxf(border, from_rising_bits(cut_down(sh, keep)));
+        if (sh.n > limit) border = fmaxf(border, from_rising_bits(cut_down(sh, keep)));
     }
     {
         const float r = warp_max(ref);
@@ -210,7 +240,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
         if (lane == 0) { sh.ref[warp] = r; sh.sum[warp] = total; }
     }
     __syncthreads();
-    if (sh.n > keep + 32) cut_down(sh, keep);
+    if (sh.n > 128 && sh.n > keep) cut_down(sh, keep);
     if (warp == 0) {
         const float w = lane < kBeamWarps ? sh.ref[lane] : -INFINITY, r = warp_max(w);
         double t = lane < kBeamWarps ? sh.sum[lane] : 0.0;
@@ -221,18 +251,14 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
     }
     // in order: every candidate's place is the number of those before it
     const int found = sh.n;
-    float* to_x = out.logits + piece * keep;
-    int* to_t = out.tokens + piece * keep;
+    u64* to = out.candidates + piece * keep;
     for (int i = tid; i < found; i += kBeamThreads) {
         const u64 key = sh.list[i];
         int before = 0;
         for (int k = 0; k < found; ++k) before += sh.list[k] > key ? 1 : 0;
-        if (before < keep) {
-            to_x[before] = from_rising_bits((unsigned)(key >> 32));
-            to_t[before] = (int)(0xffffffffu - (unsigned)key);
-        }
+        if (before < keep) to[before] = key;
     }
-    for (int i = found + tid; i < keep; i += kBeamThreads) to_t[i] = -1;
+    for (int i = found + tid; i < keep; i += kBeamThreads) to[i] = 0ull;
 }
 
 struct Candidate {
@@ -249,14 +275,16 @@ __device__ __forceinline__ bool goes_before(const Candidate& a, const Candidate&
     return a.token < b.token;
 }
 
-constexpr int kMergeKeys = 4096;
+constexpr int kMergeEach = 8, kMergeKeys = kMergeEach * kMergeThreads;
+constexpr int kMergeWarps = kMergeThreads / 32;
 struct MergeShared {
-    u64 keys[kMergeKeys];               // candidates of the lists that may hold some of the best: total rounded down to 32 bits, number
+    u64 keys[kMergeKeys];               // total (rounded down to 32 bits) and number of candidates
     double total[kMergeList];
     float logit[kMergeList];
     int beam[kMergeList], token[kMergeList];
-    int active[kMergeList];             // those lists
-    Candidate warp_best[kMergeThreads / 32];
+    int active[kMergeList];             // lists that may hold some of the best
+    Candidate warp_best[kMergeWarps];
+    int count[2][kMergeWarps];
     int n_keys, n_active, n;
 };
 
@@ -265,124 +293,137 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
                   int* __restrict__ out_beams, int* __restrict__ out_tokens) {
     extern __shared__ __align__(16) unsigned char merge_smem[];
     MergeShared& sh = *reinterpret_cast<MergeShared*>(merge_smem);
-    double* lse_s = reinterpret_cast<double*>(merge_smem + sizeof(MergeShared));        // [beams]; NaN: the row gives none
+    // [beams] what a row's sum is relative to, and the score less the sum's log (NaN: the row gives none): added to a logit in that order, so that
+    // nothing is lost where all of a row is far from 0
+    double2* offset_s = reinterpret_cast<double2*>(merge_smem + sizeof(MergeShared));
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kWarps = kMergeThreads / 32;
     if (tid == 0) sh.n = sh.n_active = sh.n_keys = 0;
     pdl_launch_dependents();
     pdl_wait();
-    for (int b = warp; b < beams; b += kWarps) {
+    const int lists = beams * chunks;       // in the order of beams
+    const long long all = (long long)lists * keep;
+    const u64* from = in.candidates + (size_t)g * all;
+    // where all candidates fit the threads' registers they are asked for before anything else
+    const bool at_once = all <= kMergeKeys;
+    u64 held[kMergeEach];
+    if (at_once) {
+#pragma unroll
+        for (int u = 0; u < kMergeEach; ++u) held[u] = tid + u * kMergeThreads < all ? from[tid + u * kMergeThreads] : 0ull;
+    }
+    for (int b = warp; b < beams; b += kMergeWarps) {
         const size_t row = (size_t)g * beams + b;
         const float score = scores[row];
-        double lse = NAN;
+        float m0 = -INFINITY;
+        double s0 = 0.0;
+        if (lane < chunks) { m0 = in.maxima[row * chunks + lane]; s0 = in.sums[row * chunks + lane]; }     // (what lies there for a row that was not read is not used)
+        double offset = NAN;
         if (fabsf(score) < INFINITY) {
-            float top = -INFINITY;
-            for (int c = lane; c < chunks; c += 32) top = fmaxf(top, in.maxima[row * chunks + c]);
+            float top = m0;
+            for (int c = lane + 32; c < chunks; c += 32) top = fmaxf(top, in.maxima[row * chunks + c]);
             top = warp_max(top);
-            double total = 0.0;
-            for (int c = lane; c < chunks; c += 32) {
+            double total = m0 > -INFINITY && m0 != top ? s0 * exp((double)m0 - (double)top) : s0;
+            for (int c = lane + 32; c < chunks; c += 32) {
                 const float mc = in.maxima[row * chunks + c];
                 const double s = in.sums[row * chunks + c];
                 total += mc > -INFINITY ? s * exp((double)mc - (double)top) : s;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-            lse = top > -INFINITY && top < INFINITY && total < (double)INFINITY ? (double)top + log(total) : NAN;    // (a NaN sum gives NaN)
+            // (a NaN sum gives NaN)
+            if (top > -INFINITY && top < INFINITY && total < (double)INFINITY) offset = (double)score - log(total);
+            m0 = top;
         }
-        if (lane == 0) lse_s[b] = lse;
+        if (lane == 0) offset_s[b] = make_double2((double)m0, offset);
     }
     __syncthreads();
 
-    const int lists = beams * chunks;       // in the order of beams
-    const size_t first_list = (size_t)g * lists;
-    auto candidate = [&](int list, int k) {
+    auto decode = [&](u64 key, int list) {
         Candidate c{-INFINITY, -INFINITY, 0, -1};
-        if (list >= lists || k >= keep) return c;
-        const int b = list / chunks;
-        const double lse = lse_s[b];
-        if (isnan(lse)) return c;
-        const size_t at = (first_list + list) * keep + k;
-        c.token = in.tokens[at];
-        if (c.token < 0) return c;
-        c.logit = in.logits[at];
-        c.beam = b;
-        c.total = (double)scores[(size_t)g * beams + b] + ((double)c.logit - lse);
+        if (key == 0ull) return c;
+        c.beam = list / chunks;
+        const double2 offset = offset_s[c.beam];
+        if (isnan(offset.y)) return c;
+        c.token = key_token(key);
+        c.logit = key_logit(key);
+        c.total = ((double)c.logit - offset.x) + offset.y;
         return c;
     };
-
-    // A number that at least `keep` candidates reach (rounded down to 32 bits) and not many more: where there are lists enough, one that `keep` of the
-    // threads' best reach; where there are few, one that so many of their (depth + 1)-th best reach that it comes to as much.  None: all candidates.
-    bool head = false;
-    for (int l = tid; l < lists; l += kMergeThreads) head = head || candidate(l, 0).token >= 0;
-    const int n_heads = __syncthreads_count(head);
-    const int depth = n_heads >= keep || n_heads == 0 ? 0 : (2 * keep + n_heads - 1) / n_heads - 1, need = (keep + depth) / (depth + 1);
-    unsigned key = 0;
-    for (int l = tid; l < lists; l += kMergeThreads) {
-        const Candidate c = candidate(l, depth);
-        if (c.token >= 0) key = max(key, rising_bits(__double2float_rd(c.total)));
-    }
-    unsigned least = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned t = least | (1u << bit);
-        const int n = __syncthreads_count(key >= t);
-        if (n >= need) least = t;
-        if (n >= need && n <= need + need / 4) break;
-    }
-    least = max(least, 1u);
-    // the lists with a candidate that reaches it, a thread each; then of those, a warp each, all that reach it
-    for (int l = tid; l < lists; l += kMergeThreads) {
-        const Candidate c = candidate(l, 0);
-        if (c.token >= 0 && rising_bits(__double2float_rd(c.total)) >= least) {
-            const int i = atomicAdd(&sh.n_active, 1);
-            if (i < kMergeList) sh.active[i] = l;
-        }
-    }
-    __syncthreads();
-    const int n_active = sh.n_active;
-    for (int a = warp; a < min(n_active, kMergeList); a += kWarps) {
-        for (int k0 = 0; k0 < keep; k0 += 32) {
-            const Candidate c = candidate(sh.active[a], k0 + lane);
-            const unsigned b = rising_bits(__double2float_rd(c.total));
-            const bool in = c.token >= 0 && b >= least;
-            if (in) {
-                const int i = atomicAdd(&sh.n_keys, 1);
-                if (i < kMergeKeys) sh.keys[i] = ((u64)b << 32) | (unsigned)(sh.active[a] * keep + k0 + lane);
+    auto candidate = [&](int list, int k) { return decode(list < lists && k < keep ? from[(size_t)list * keep + k] : 0ull, list); };
+    // a candidate's total rounded down to 32 bits, as a number that rises with it; 0: none
+    auto rounded = [&](const Candidate& c) { return c.token >= 0 ? rising_bits(__double2float_rd(c.total)) : 0u; };
+    // the largest number that `need` of all threads' keys reach (0: there are not as many), or one that few more do
+    auto search = [&](auto count_mine, int need) {
+        unsigned least = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const unsigned t = least | (1u << bit);
+            int n = __reduce_add_sync(0xffffffffu, count_mine(t));
+            if (lane == 0) sh.count[bit & 1][warp] = n;     // (two sets of counts in turn: one barrier a count)
+            __syncthreads();
+            n = __reduce_add_sync(0xffffffffu, lane < kMergeWarps ? sh.count[bit & 1][lane] : 0);
+            if (n >= need) {
+                least = t;
+                if (n <= need + need / 4) break;
             }
-            if (!__any_sync(0xffffffffu, in)) break;
         }
-    }
-    __syncthreads();
-    const int n_keys = sh.n_keys;
-    if (n_active <= kMergeList && n_keys <= kMergeKeys) {
-        constexpr int kEach = kMergeKeys / kMergeThreads;
-        u64 mine[kEach];
+        return max(least, 1u);
+    };
+    unsigned least = 1;
+    bool listed = true;         // what may be among the best has gone to the list
+    u64 mine[kMergeEach];       // total and number
+    if (at_once) {
 #pragma unroll
-        for (int u = 0; u < kEach; ++u) mine[u] = tid + u * kMergeThreads < n_keys ? sh.keys[tid + u * kMergeThreads] : 0ull;
-        if (n_keys > keep + keep / 4) {     // the same search over all of these
-            least = 0;
-            for (int bit = 31; bit >= 0; --bit) {
-                const unsigned t = least | (1u << bit);
-                int n = 0;
-#pragma unroll
-                for (int u = 0; u < kEach; ++u) n += (unsigned)(mine[u] >> 32) >= t ? 1 : 0;
-                n = __reduce_add_sync(0xffffffffu, n);
-                __shared__ int count[2][kWarps];
-                if (lane == 0) count[bit & 1][warp] = n;
-                __syncthreads();
-                n = 0;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) n += count[bit & 1][w];
-                if (n >= keep) {
-                    least = t;
-                    if (n <= keep + keep / 4) break;
+        for (int u = 0; u < kMergeEach; ++u) {
+            const int i = tid + u * kMergeThreads;
+            mine[u] = ((u64)rounded(decode(held[u], i / keep)) << 32) | (unsigned)i;
+        }
+    } else {
+        // A number that at least `keep` candidates reach and not many more: where there are lists enough, one that `keep` of the threads'
+        // best heads reach; where there are few, one that so many of their (depth + 1)-th best reach that it comes to as much.
+        bool head = false;
+        for (int l = tid; l < lists; l += kMergeThreads) head = head || candidate(l, 0).token >= 0;
+        const int n_heads = __syncthreads_count(head);
+        const int depth = n_heads >= keep || n_heads == 0 ? 0 : (2 * keep + n_heads - 1) / n_heads - 1;
+        unsigned key = 0;
+        for (int l = tid; l < lists; l += kMergeThreads) key = max(key, rounded(candidate(l, depth)));
+        least = search([&](unsigned t) { return key >= t ? 1 : 0; }, (keep + depth) / (depth + 1));
+        __syncthreads();
+        // the lists with a candidate that reaches it, a thread each; then of those, a warp each, all that reach it
+        for (int l = tid; l < lists; l += kMergeThreads) {
+            if (rounded(candidate(l, 0)) >= least) {
+                const int i = atomicAdd(&sh.n_active, 1);
+                if (i < kMergeList) sh.active[i] = l;
+            }
+        }
+        __syncthreads();
+        const int n_active = sh.n_active;
+        for (int a = warp; a < min(n_active, kMergeList); a += kMergeWarps) {
+            for (int k0 = 0; k0 < keep; k0 += 32) {
+                const unsigned b = rounded(candidate(sh.active[a], k0 + lane));
+                const bool in = b >= least;
+                if (in) {
+                    const int i = atomicAdd(&sh.n_keys, 1);
+                    if (i < kMergeKeys) sh.keys[i] = ((u64)b << 32) | (unsigned)(sh.active[a] * keep + k0 + lane);
                 }
+                if (!__any_sync(0xffffffffu, in)) break;
             }
         }
+        __syncthreads();
+        listed = n_active <= kMergeList && sh.n_keys <= kMergeKeys;
 #pragma unroll
-        for (int u = 0; u < kEach; ++u) {
-            if ((unsigned)(mine[u] >> 32) >= max(least, 1u)) {
+        for (int u = 0; u < kMergeEach; ++u) mine[u] = tid + u * kMergeThreads < min(sh.n_keys, kMergeKeys) ? sh.keys[tid + u * kMergeThreads] : 0ull;
+    }
+    if (listed) {
+        least = search([&](unsigned t) {
+            int n = 0;
+#pragma unroll
+            for (int u = 0; u < kMergeEach; ++u) n += (unsigned)(mine[u] >> 32) >= t ? 1 : 0;
+            return n;
+        }, keep);
+#pragma unroll
+        for (int u = 0; u < kMergeEach; ++u) {
+            if ((unsigned)(mine[u] >> 32) >= least) {
                 const unsigned number = (unsigned)mine[u];
-                const Candidate c = candidate(number / keep, number % keep);
+                const Candidate c = at_once ? decode(held[u], number / keep) : candidate(number / keep, number % keep);
                 const int i = atomicAdd(&sh.n, 1);
                 if (i < kMergeList) { sh.total[i] = c.total; sh.logit[i] = c.logit; sh.beam[i] = c.beam; sh.token[i] = c.token; }
             }
@@ -390,7 +431,7 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
     }
     __syncthreads();
     const size_t to = (size_t)g * keep;
-    const int found = n_active <= kMergeList && n_keys <= kMergeKeys ? sh.n : kMergeList + 1;
+    const int found = listed ? sh.n : kMergeList + 1;
     if (found <= kMergeList) {
         for (int i = tid; i < found; i += kMergeThreads) {
             const Candidate c{sh.total[i], sh.logit[i], sh.beam[i], sh.token[i]};
@@ -439,7 +480,7 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         if (lane == 0) sh.warp_best[warp] = best;
         __syncthreads();
         best = sh.warp_best[0];
-        for (int w = 1; w < kWarps; ++w) if (goes_before(sh.warp_best[w], best)) best = sh.warp_best[w];
+        for (int w = 1; w < kMergeWarps; ++w) if (goes_before(sh.warp_best[w], best)) best = sh.warp_best[w];
         __syncthreads();
         last = best;
         if (tid == 0) {
@@ -487,12 +528,12 @@ extern "C" int b200_beam_select(const float* logits, long long ld, const float* 
     if (scratch_bytes < b200_beam_select_scratch_bytes((int)rows, vocab, keep)) return 10003;
     const BeamScratch s = beam_scratch(scratch, rows * chunks, keep);
     const int vec = ((uintptr_t)logits & 15) == 0 && (ld & 3) == 0;
-    const size_t merge_bytes = sizeof(MergeShared) + sizeof(double) * beams;
+    const size_t merge_bytes = sizeof(MergeShared) + sizeof(double2) * beams;
     static bool configured[64] = {};
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
     if (!configured[device]) {
-        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(MergeShared) + 8 * 1024));
+        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(MergeShared) + sizeof(double2) * 1024));
         if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
         configured[device] = true;
     }

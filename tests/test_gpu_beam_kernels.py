@@ -25,10 +25,10 @@ def _reference(logits, scores, n):
     G, B = scores.shape
     x = logits.double().cpu().view(G, B, -1)
     m = x.amax(-1, keepdim=True)
-    lse = m + torch.log(torch.exp(x - m).sum(-1, keepdim=True))
+    log_sum = torch.log(torch.exp(x - m).sum(-1, keepdim=True))
     s = scores.double().cpu().unsqueeze(-1)
-    total = s + (x - lse)
-    total[~(torch.isfinite(s) & torch.isfinite(lse)).expand_as(total)] = -INF
+    total = s + ((x - m) - log_sum)         # (not x - (m + log_sum): at the type's lowest value that loses the second)
+    total[~(torch.isfinite(s) & torch.isfinite(m + log_sum)).expand_as(total)] = -INF
     total[x == -INF] = -INF
     order = []
     for g in range(G):
