@@ -3,7 +3,8 @@
 A page holds the keys and values of ``PAGE_TOKENS`` consecutive positions of one sequence (for
 every cache entry of its group).  Pages and slots are handed out from free lists and must come
 back exactly once; both allocators refuse a double free or a foreign id, which is what the
-cache tests lean on (no page or slot lost, held twice or freed twice)."""
+cache tests lean on (no page or slot lost, held twice or freed twice).  A page may have several
+holders (sequences that began as one): it comes back once from each, and is free after the last."""
 from __future__ import annotations
 
 PAGE_TOKENS = 64
@@ -27,7 +28,7 @@ class PagePool:
             raise ValueError("n_pages must be >= 0")
         self.n_pages = n_pages
         self._free = list(range(n_pages - 1, -1, -1))  # pop() hands out low ids first
-        self._held = [False] * n_pages
+        self._holders = [0] * n_pages
 
     @property
     def n_free(self) -> int:
@@ -42,18 +43,28 @@ class PagePool:
             raise CacheFull(f"need {n} cache page(s) of {PAGE_TOKENS} tokens, {len(self._free)} of {self.n_pages} free")
         out = [self._free.pop() for _ in range(n)]
         for p in out:
-            self._held[p] = True
+            self._holders[p] = 1
         return out
+
+    def holders(self, page: int) -> int:
+        return self._holders[page]
+
+    def share(self, pages) -> None:
+        """Each of ``pages`` gets one holder more."""
+        for p in pages:
+            if not (0 <= p < self.n_pages) or self._holders[p] == 0:
+                raise CacheError(f"page {p} is not held and cannot be shared")
+            self._holders[p] += 1
 
     def free(self, pages) -> None:
         pages = list(pages)
         for p in pages:
             if not (0 <= p < self.n_pages):
                 raise CacheError(f"page {p} does not belong to this pool of {self.n_pages}")
-            if not self._held[p]:
+            if self._holders[p] == 0:
                 raise CacheError(f"page {p} freed twice")
-            self._held[p] = False
-        self._free.extend(reversed(pages))
+            self._holders[p] -= 1
+        self._free.extend(p for p in reversed(pages) if self._holders[p] == 0)
 
 
 class SlotTable:

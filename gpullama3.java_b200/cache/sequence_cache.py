@@ -21,7 +21,9 @@ sequence (inference/state/LlamaState.java:44-46,61-64 of the reference project).
   a tuple of named needs: each goes to the group of its kind and the block is handed a dict of views;
 * a *slot* is acquired when a sequence starts and released when it ends; its pages go back to
   the pools and are handed to later sequences without clearing (positions at or beyond a
-  sequence's length are never read).
+  sequence's length are never read);
+* a sequence may be *forked*: the new one shares the pages written so far and gets copies of the states of fixed size.  A
+  page that is not full is copied when one of its holders is about to write (``reserve``), for all of them but the last.
 """
 from __future__ import annotations
 
@@ -29,6 +31,7 @@ from dataclasses import dataclass
 
 import torch
 
+from ..kernels import ops
 from .pages import PAGE_TOKENS, CacheError, CacheFull, PagePool, SlotTable, pages_for
 
 
@@ -76,6 +79,7 @@ class CacheGroup:
     """Storage of the cache entries that share one need.  ``paged`` groups grow with their sequences and
     have a page table in every step's context; the others have a fixed size per slot."""
     paged = False
+    can_fork = False   # whether a sequence's part of it can be handed on to a second one (``copy``, in a paged group for its pages)
 
     def __init__(self, need, entries: list[int], sizes: CacheSizes):
         self.need, self.entries = need, list(entries)
@@ -87,6 +91,10 @@ class CacheGroup:
 
     def release(self, slot: int) -> None:
         """The sequence in ``slot`` is over."""
+
+    def copy(self, moves) -> None:
+        """Copies storage on the device: of states (source slot, destination slot), of pages (source, destination, positions in use)."""
+        raise NotImplementedError
 
     def view(self, entry: int):
         """What the mixer of ``entry`` is handed in ``forward``."""
@@ -119,9 +127,19 @@ class PagedGroup(CacheGroup):
         self.pool = PagePool(n_pages)
         # per live slot: logical page index -> physical page, -1 where a windowed group let go
         self.rows: dict[int, list[int]] = {}
+        self._stamp, self._stamps = 0, {}
+
+    def stamp(self, slot: int) -> int:
+        """A number that no other row has had: it changes whenever the slot's row of pages does."""
+        return self._stamps[slot]
+
+    def _changed(self, slot: int) -> None:
+        self._stamp += 1
+        self._stamps[slot] = self._stamp
 
     def acquire(self, slot):
         self.rows[slot] = []
+        self._changed(slot)
 
     def release(self, slot):
         self.pool.free([p for p in self.rows.pop(slot) if p >= 0])
@@ -133,6 +151,42 @@ class PagedGroup(CacheGroup):
         extra = self.pages_needed(slot, new_length)
         if extra > 0:
             self.rows[slot].extend(self.pool.alloc(extra))
+            self._changed(slot)
+
+    def fork(self, slot: int, new_slot: int, length: int) -> None:
+        """A new sequence in ``new_slot`` shares the pages that ``slot`` has written."""
+        row = self.rows[slot][:pages_for(length)]
+        self.pool.share([p for p in row if p >= 0])
+        self.rows[new_slot] = row
+        self._changed(new_slot)
+
+    def shared_writes(self, slots, lengths: dict[int, int]) -> int:
+        """How many pages must be copied before all of ``slots`` (each once) are written to behind their lengths."""
+        writers: dict[int, int] = {}
+        for s in slots:
+            page = self._open_page(s, lengths[s])
+            if page is not None:
+                writers[page] = writers.get(page, 0) + 1
+        return sum(min(n, self.pool.holders(p) - 1) for p, n in writers.items())
+
+    def make_own(self, slots, lengths: dict[int, int]) -> list[tuple[int, int, int]]:
+        """Gives each of ``slots`` a page of its own for the positions behind its length where that page has other holders; the
+        copies this takes, as (source, destination, positions in use)."""
+        moves = []
+        for s in slots:
+            page = self._open_page(s, lengths[s])
+            if page is not None and self.pool.holders(page) > 1:
+                own = self.pool.alloc(1)[0]
+                self.pool.free([page])
+                self.rows[s][lengths[s] // PAGE_TOKENS] = own
+                self._changed(s)
+                moves.append((page, own, lengths[s] % PAGE_TOKENS))
+        return moves
+
+    def _open_page(self, slot: int, length: int) -> int | None:
+        """The page that is neither empty nor full, if there is one."""
+        row, at = self.rows[slot], length // PAGE_TOKENS
+        return row[at] if length % PAGE_TOKENS and at < len(row) and row[at] >= 0 else None
 
     def commit(self, slot: int, new_length: int) -> None:
         """The sequence now holds ``new_length`` tokens: let go of pages no later query can reach."""
@@ -149,11 +203,17 @@ class PagedGroup(CacheGroup):
             self.pool.free(drop)
             for i in range(self.kept_pages, dead):
                 row[i] = -1
+            self._changed(slot)
 
     def check(self):
-        held = [p for row in self.rows.values() for p in row if p >= 0]
-        if len(held) != len(set(held)):
-            raise CacheError(f"paged group {self.index}: a page is held twice")
+        held: dict[int, int] = {}
+        for row in self.rows.values():
+            for p in row:
+                if p >= 0:
+                    held[p] = held.get(p, 0) + 1
+        for p, n in held.items():
+            if n != self.pool.holders(p):
+                raise CacheError(f"paged group {self.index}: page {p} is held {n} time(s), its holders are {self.pool.holders(p)}")
         if len(held) != self.pool.n_held:
             raise CacheError(f"paged group {self.index}: {self.pool.n_held} pages are out but slots hold {len(held)}")
 
@@ -170,6 +230,8 @@ class KVView:
 
 
 class KVGroup(PagedGroup):
+    can_fork = True
+
     def __init__(self, need: KVCacheNeed, entries, sizes: CacheSizes):
         super().__init__(need, entries, sizes, window=need.window, keep_first=need.keep_first, chunk=need.chunk)
         n = self.pool.n_pages
@@ -179,6 +241,14 @@ class KVGroup(PagedGroup):
         self.v = torch.zeros((len(self.entries), n, need.n_kv_heads, need.head_dim, PAGE_TOKENS), dtype=sizes.dtype,
                              device=sizes.device)
         self.work_counters = torch.zeros(4, dtype=torch.int32, device=sizes.device)
+
+    def copy(self, moves):
+        if self.k.is_cuda:
+            ops.copy_pages(self.k, self.v, moves)
+            return
+        for s, d, n in moves:   # (a cache without a GPU: its bookkeeping is what is used)
+            self.k[:, d, :, :n] = self.k[:, s, :, :n]
+            self.v[:, d, :, :, :n] = self.v[:, s, :, :, :n]
 
     def view(self, entry):
         i = self.entry_pos[entry]
@@ -195,12 +265,21 @@ class StateView:
 
 
 class StateGroup(CacheGroup):
+    can_fork = True
+
     def __init__(self, need: StateNeed, entries, sizes: CacheSizes):
         super().__init__(need, entries, sizes)
         self.data = torch.zeros((len(self.entries), sizes.max_slots, *need.shape), dtype=need.dtype, device=sizes.device)
 
     def acquire(self, slot):
         self.data[:, slot].zero_()
+
+    def copy(self, moves):
+        if self.data.is_cuda:
+            ops.copy_slots(self.data, moves)
+            return
+        for s, d in moves:
+            self.data[:, d] = self.data[:, s]
 
     def view(self, entry):
         return StateView(data=self.data[self.entry_pos[entry]])
@@ -272,7 +351,8 @@ class SequenceCache:
             for e in entries:
                 self._entry_group[e] = g
         self._length: dict[int, int] = {}
-        # counts acquisitions and releases: while it stands still, a slot number means the same sequence
+        # counts acquisitions and releases, and pages exchanged for copies: while it stands still, a slot number means the same
+        # sequence and its pages are the ones it had (and more, as it grows)
         self.ownership_changes = 0
 
     @property
@@ -297,6 +377,82 @@ class SequenceCache:
             g.release(slot)
         self.slots.release(slot)
 
+    def fork(self, slots: list[int]) -> list[int]:
+        """A new sequence for each of ``slots`` (a slot may come several times), each continuing that slot's: it shares the pages
+        written so far, and the states of fixed size are copied.  Returns the new slots.  Nothing changes if there are too few."""
+        for slot in slots:
+            if slot not in self._length:
+                raise CacheError(f"slot {slot} is not live")
+        if not slots:
+            return []
+        self._check_can_fork()
+        if len(slots) > self.slots.n_free:
+            raise CacheFull(f"{len(slots)} sequence slot(s) needed, {self.slots.n_free} of {self.max_slots} are free")
+        moves = []
+        for slot in slots:
+            new = self.slots.acquire()
+            self.ownership_changes += 1
+            self._length[new] = self._length[slot]
+            for g in self.paged_groups:
+                g.fork(slot, new, self._length[slot])
+            moves.append((slot, new))
+        for g in self.slot_groups:
+            g.copy(moves)
+        return [new for _, new in moves]
+
+    def _check_can_fork(self) -> None:
+        for g in self.groups:
+            if not g.can_fork:
+                raise CacheError(f"a cache with {type(g).__name__} cannot fork its sequences")
+
+    def reorder(self, slots: list[int], parents: list[int]) -> list[int]:
+        """The sequences of ``slots`` go on as the children named by ``parents``: child i continues slots[parents[i]].  A sequence without
+        children is over, one with children goes on as one of them (child i itself, if it is among them) and is forked for
+        the others.  Returns the children's slots; no more of them are needed than there were."""
+        if len(parents) > len(slots) or len(set(slots)) != len(slots):
+            raise CacheError(f"{len(parents)} children of the slots {slots}")
+        for slot in slots:
+            if slot not in self._length:
+                raise CacheError(f"slot {slot} is not live")
+        if any(not 0 <= p < len(slots) for p in parents):
+            raise CacheError(f"parents {parents} of {len(slots)} sequences")
+        keeper = {}             # parent -> the child that goes on in its slot
+        for child, p in enumerate(parents):
+            if p not in keeper or child == p:
+                keeper[p] = child
+        if len(keeper) < len(parents):
+            self._check_can_fork()
+        for p, slot in enumerate(slots):
+            if p not in keeper:
+                self.release(slot)
+        others = [child for child, p in enumerate(parents) if keeper[p] != child]
+        new = dict(zip(others, self.fork([slots[parents[child]] for child in others])))
+        return [new[child] if child in new else slots[p] for child, p in enumerate(parents)]
+
+    def shared_pages(self, slots: list[int]) -> list[int]:
+        """Per paged group, how many of the first full pages are the same for all of ``slots``."""
+        lengths = [self._length[s] for s in slots]
+        n_full = min(lengths) // PAGE_TOKENS
+        out = []
+        for g in self.paged_groups:
+            rows = [g.rows[s] for s in slots]
+            first = rows[0]
+            if min(lengths) == max(lengths):
+                # a page that all hold came to them with everything before it: the common ones end at one place
+                lo, hi = 0, n_full
+                while lo < hi:
+                    mid = (lo + hi) // 2
+                    if all(r[mid] == first[mid] for r in rows):
+                        lo = mid + 1
+                    else:
+                        hi = mid
+            else:                       # (a window may have let go of a page in one and not in the other)
+                lo = 0
+                while lo < n_full and all(r[lo] == first[lo] for r in rows):
+                    lo += 1
+            out.append(lo)
+        return out
+
     def length(self, slot: int) -> int:
         return self._length[slot]
 
@@ -314,10 +470,17 @@ class SequenceCache:
         for slot, _ in requests:
             if slot not in self._length:
                 raise CacheError(f"slot {slot} is not live")
+        writers = list(dict.fromkeys(slot for slot, n_new in requests if n_new > 0))
         for g, n in zip(self.paged_groups, self.pages_needed(requests)):
+            n += g.shared_writes(writers, self._length)
             if n > g.pool.n_free:
                 raise CacheFull(f"cache group {g.index} needs {n} more page(s) of {PAGE_TOKENS} tokens, "
                                 f"{g.pool.n_free} of {g.pool.n_pages} are free")
+        for g in self.paged_groups:
+            moves = g.make_own(writers, self._length)
+            if moves:
+                self.ownership_changes += 1
+                g.copy(moves)
         for slot, n_new in requests:
             for g in self.paged_groups:
                 g.reserve(slot, self._length[slot] + n_new)
@@ -350,7 +513,7 @@ class SequenceCache:
         return sum(g.bytes_per_token() for g in self.paged_groups)
 
     def check_invariants(self) -> None:
-        """Every page is free or held by exactly one live slot; used by tests."""
+        """Every page is free or held by the live slots that its holders count; used by tests."""
         for g in self.groups:
             g.check()
             if g.paged and set(g.rows) != set(self._length):
