@@ -4,6 +4,7 @@ generation loop.
     engine = Engine.from_folder("model_dir", dtype="bfloat16", max_tokens=32768)
     outputs = engine.generate([[1, 2, 3], [4, 5]], max_new_tokens=16)          # greedy
     outputs = engine.generate(prompts, max_new_tokens=16, temperature=0.8, seed=1)
+    outputs = engine.beam_search(prompts, beams=4, max_new_tokens=16)                    # the most probable continuations
 
 Token ids go in and come out as Python lists; everything between runs on the GPU."""
 from __future__ import annotations
@@ -16,6 +17,7 @@ from ..cache.pages import PAGE_TOKENS
 from ..config.base import ModelConfig, read_config_json
 from ..config.registry import architecture_of
 from ..sampling.sampler import Sampler, SamplingParams
+from .beams import BeamHypothesis, BeamParams, BeamSearcher
 from .generate import GenerationResult, Generator
 from .step import SequenceInput, StepFunction
 
@@ -88,6 +90,8 @@ class Engine:
         self.stop_ids: tuple[int, ...] = tuple(self.config.stop_token_ids)
         self.generator = Generator(_LoopStep(self.step_fn), self.cache, Sampler, max_batch=max_batch,
                                    max_length=self.max_length)
+        self.searcher = BeamSearcher(self.step_fn, self.cache, max_batch=max_batch, max_length=self.max_length)
+        self._last_run = self.generator
 
     # ---- construction
     @classmethod
@@ -121,14 +125,30 @@ class Engine:
             stop_ids = self.stop_ids
         results = self.generator.generate([list(p) for p in prompts], max_new_tokens,
                                           SamplingParams(temperature, top_p, seed), stop_ids, on_token)
+        self._last_run = self.generator
         return results if return_results else [r.tokens for r in results]
+
+    def beam_search(self, prompts: list[list[int]], beams: int = 4, max_new_tokens: int = 16, *, length_penalty: float = 1.0,
+                    n_best: int = 1, stop_ids=None, return_hypotheses: bool = False):
+        """The most probable continuation found per prompt with ``beams`` beams (token ids, the stop token included when one ended it); with
+        ``n_best`` > 1 a list of so many per prompt, the best first.  Hypotheses are ranked by the sum of their tokens' log
+        probabilities over their length to the power of ``length_penalty``.  ``return_hypotheses``: ``BeamHypothesis`` records, with
+        log probability, score and finish reason, in place of token ids.  A batch takes ``beams`` sequences of ``max_batch``
+        per request."""
+        if stop_ids is None:
+            stop_ids = self.stop_ids
+        found = self.searcher.search([list(p) for p in prompts], max_new_tokens, BeamParams(beams, length_penalty, n_best), stop_ids)
+        self._last_run = self.searcher
+        if not return_hypotheses:
+            found = [[h.tokens for h in hyps] for hyps in found]
+        return [hyps[0] for hyps in found] if n_best == 1 else found
 
     @property
     def last_metrics(self):
-        return self.generator.last_metrics
+        return self._last_run.last_metrics
 
     def step(self, inputs: list[SequenceInput]) -> torch.Tensor | None:
         return self.step_fn(inputs)
 
 
-__all__ = ["Engine", "GenerationResult", "SequenceInput", "SamplingParams"]
+__all__ = ["BeamHypothesis", "Engine", "GenerationResult", "SequenceInput", "SamplingParams"]

@@ -51,6 +51,11 @@ def create_parser() -> argparse.ArgumentParser:
     g.add_argument("-sp", "--system-prompt", type=parse_token_ids, help="token ids put before every prompt")
     g.add_argument("--temperature", "--temp", type=float, default=0.1, help="softmax temperature of the draw; 0 takes the arg-max")
     g.add_argument("--top-p", type=float, default=0.95, help="probability mass of the nucleus a token is drawn from; 0 or 1: all tokens")
+    g.add_argument("--beams", type=int, default=1,
+                   help="more than 1: beam search with so many beams per request in place of drawing tokens (--temperature, --top-p, --seed "
+                        "and --stream do not apply; each beam counts against --max-batch)")
+    g.add_argument("--length-penalty", type=float, default=1.0,
+                   help="with --beams: hypotheses are ranked by log probability / length ** this")
     g.add_argument("--seed", "-s", type=int, default=None, help="seed of the draws (when absent: the clock, printed with --verbose-init)")
     g.add_argument("-n", "--max-tokens", type=int, default=512, help="most new tokens per request")
     g.add_argument("--max-len", type=int, default=None,
@@ -117,6 +122,10 @@ def main(argv=None) -> int:
         parser.error("--interactive: the chat mode needs a tokenizer and is not part of this library")
     if args.suffix:
         parser.error("--suffix: fill-in-the-middle is not part of this library")
+    if args.beams < 1:
+        parser.error("--beams must be at least 1")
+    if args.beams > args.max_batch:
+        parser.error(f"--beams {args.beams} needs --max-batch {args.beams} at least")
     if args.temperature < 0:
         parser.error("--temperature must be non-negative")
     if not (0 <= args.top_p <= 1):
@@ -134,7 +143,9 @@ def main(argv=None) -> int:
     if args.system_prompt:
         prompts = [args.system_prompt + p for p in prompts]
     seed = args.seed if args.seed is not None else int(time.time())
-    need = sum(-(-(len(p) + args.max_tokens) // 64) * 64 for p in prompts[:args.max_batch])
+    # (a beam search: as if no beam shared the prompt's pages)
+    longest = [-(-(len(p) + args.max_tokens) // 64) * 64 for p in prompts]
+    need = args.beams * max(sum(longest[:args.max_batch // args.beams]), max(longest) if args.beams > 1 else 0)
     cache_tokens = args.cache_tokens or max(need, 64)
 
     if args.show_config:
@@ -152,7 +163,7 @@ def main(argv=None) -> int:
     if args.show_command:
         print(json.dumps({"model": args.model_path, "config": args.config, "random_weights": args.random_weights,
                           "dtype": args.dtype, "prompts": len(prompts), "temperature": args.temperature,
-                          "top_p": args.top_p, "seed": seed, "max_tokens": args.max_tokens,
+                          "top_p": args.top_p, "seed": seed, "beams": args.beams, "max_tokens": args.max_tokens,
                           "max_len": args.max_len, "cache_tokens": cache_tokens, "max_batch": args.max_batch}, indent=2))
         if not args.execute_after_show:
             return 0
@@ -179,7 +190,7 @@ def main(argv=None) -> int:
         for p in prompts:
             print(" ".join(map(str, p)), file=sys.stderr)
 
-    single = len(prompts) == 1
+    single = len(prompts) == 1 and args.beams == 1
 
     def on_token(i, tok):
         if args.echo:
@@ -187,8 +198,11 @@ def main(argv=None) -> int:
         if args.stream and single:
             print(tok, end=" ", flush=True)
 
-    outs = engine.generate(prompts, max_new_tokens=args.max_tokens, temperature=args.temperature, top_p=args.top_p,
-                           seed=seed, stop_ids=args.stop, on_token=on_token)
+    if args.beams > 1:
+        outs = engine.beam_search(prompts, args.beams, args.max_tokens, length_penalty=args.length_penalty, stop_ids=args.stop)
+    else:
+        outs = engine.generate(prompts, max_new_tokens=args.max_tokens, temperature=args.temperature, top_p=args.top_p,
+                               seed=seed, stop_ids=args.stop, on_token=on_token)
     if args.stream and single:
         print()
     else:

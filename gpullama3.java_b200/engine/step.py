@@ -54,7 +54,13 @@ def _pack(cache: SequenceCache, slots, start_pos, token_lists, logit_rows, width
     return pieces, q_lens, [t.shape for t in tables]
 
 
-def _context_over(dev: torch.Tensor, sizes, table_shapes, dtype, device, slots, start_pos, q_lens, kv_capacity=None):
+def _shared_pages(cache: SequenceCache, slots: list[int], beams: int) -> np.ndarray:
+    """Per paged group and group of ``beams`` sequences, how many first pages its sequences have in common."""
+    per_group = [cache.shared_pages(slots[i:i + beams]) for i in range(0, len(slots), beams)]
+    return np.asarray(per_group, dtype=np.int32).reshape(len(per_group), len(cache.paged_groups)).T.reshape(-1)
+
+
+def _context_over(dev: torch.Tensor, sizes, table_shapes, dtype, device, slots, start_pos, q_lens, kv_capacity=None, beams: int = 1):
     views, off = [], 0
     for n in sizes:
         views.append(dev[off:off + n])
@@ -64,21 +70,25 @@ def _context_over(dev: torch.Tensor, sizes, table_shapes, dtype, device, slots, 
         start_pos=list(start_pos), q_lens=list(q_lens), all_decode=all(q == 1 for q in q_lens), max_q_len=max(q_lens),
         max_kv_len=max(s + q for s, q in zip(start_pos, q_lens)), tokens=views[0], positions=views[1],
         seq_ids=views[2], cu_seqlens=views[3], kv_lens=views[4], slots_dev=views[5],
-        page_tables=[v.view(shape) for v, shape in zip(views[7:], table_shapes)])
+        page_tables=[v.view(shape) for v, shape in zip(views[7:7 + len(table_shapes)], table_shapes)])
+    if beams > 1:
+        ctx.beams, ctx.shared_pages = beams, list(views[7 + len(table_shapes)].view(len(table_shapes), len(slots) // beams))
     ctx.kv_capacity = list(kv_capacity) if kv_capacity is not None else [ctx.max_kv_len] * len(table_shapes)
     return ctx, views[6]
 
 
 def build_context(dtype, device, cache: SequenceCache, slots: list[int], start_pos: list[int],
-                  token_lists: list, logit_rows: list[int], workspace=None) -> tuple[StepContext, torch.Tensor | None]:
+                  token_lists: list, logit_rows: list[int], workspace=None, beams: int = 1) -> tuple[StepContext, torch.Tensor | None]:
     """Pack one pass into a StepContext.  All integers go to the device in one copy.  ``workspace``: where the
-    pass takes its intermediate tensors from (it is reset here)."""
+    pass takes its intermediate tensors from (it is reset here).  ``beams``: the sequences come in groups of so many that began as one."""
     pieces, q_lens, table_shapes = _pack(cache, slots, start_pos, token_lists, logit_rows)
+    if beams > 1:
+        pieces.append(_shared_pages(cache, slots, beams))
     host = torch.from_numpy(np.concatenate(pieces))
     if device.type == "cuda":
         host = host.pin_memory()
     dev = host.to(device, non_blocking=True)
-    ctx, rows = _context_over(dev, [p.size for p in pieces], table_shapes, dtype, device, slots, start_pos, q_lens)
+    ctx, rows = _context_over(dev, [p.size for p in pieces], table_shapes, dtype, device, slots, start_pos, q_lens, beams=beams)
     ctx.extras["host_buffer"] = host  # keep the pinned source alive until the copy has run
     if workspace is not None:
         workspace.reset()
@@ -119,21 +129,26 @@ class DecodeGraph:
     project)."""
 
     def __init__(self, model, cache: SequenceCache, n_seqs: int, widths: list[int], sampler=None,
-                 tokens_dev: torch.Tensor | None = None, fed: bool = False):
-        """``tokens_dev``: where the draw leaves its tokens on the device (its own buffer if none is given).
+                 tokens_dev: torch.Tensor | None = None, fed: bool = False, beams: int = 1):
+        """``beams``: the sequences come in groups of so many that began as one (``StepContext.beams``).  ``tokens_dev``: where the draw leaves its tokens on the device (its own buffer if none is given).
         ``fed``: the step's input tokens are what ``tokens_dev`` holds when the step starts, i.e. the tokens the
         step before it drew for the same sequences; the host then stages positions and page tables only."""
         self.model, self.cache, self.n, self.widths = model, cache, n_seqs, list(widths)
         self.sampler = sampler                        # its launches are recorded after the model's, if given
-        self.fed = bool(fed)
+        self.fed, self.beams = bool(fed), beams
         assert not fed or (sampler is not None and tokens_dev is not None)
         self.draws = sampler is not None and sampler.uniforms([0], [0]) is not None
+        n_out = sampler.outputs(n_seqs) if hasattr(sampler, "outputs") else n_seqs
         self.sizes = [n_seqs, n_seqs, n_seqs, n_seqs + 1, n_seqs, n_seqs, n_seqs] + [n_seqs * w for w in widths]
         self.table_shapes = [(n_seqs, w) for w in widths]
         self.table_offsets, off = [], sum(self.sizes[:7])
         for w in widths:
             self.table_offsets.append(off)
             off += n_seqs * w
+        self.shared_offset = off                      # of a beam search's step: counts of shared pages
+        if beams > 1:
+            self.sizes.append(len(widths) * (n_seqs // beams))
+            off += self.sizes[-1]
         self.uniform_offset = off                     # float32 numbers of the draws, after the integers
         total = off + (n_seqs if self.draws else 0)
         self.host = torch.empty(total, dtype=torch.int32).pin_memory()
@@ -142,21 +157,22 @@ class DecodeGraph:
         if sampler is None:
             self.tokens_dev = None
         elif tokens_dev is not None:
-            assert tokens_dev.shape == (n_seqs,) and tokens_dev.dtype == torch.int32
+            assert tokens_dev.shape == (n_out,) and tokens_dev.dtype == torch.int32
             self.tokens_dev = tokens_dev
         else:
-            self.tokens_dev = torch.empty(n_seqs, dtype=torch.int32, device=model.device)
-        self.tokens_host = torch.empty(n_seqs, dtype=torch.int32).pin_memory() if sampler is not None else None
+            self.tokens_dev = torch.empty(n_out, dtype=torch.int32, device=model.device)
+        self.tokens_host = torch.empty(n_out, dtype=torch.int32).pin_memory() if sampler is not None else None
         self.done = torch.cuda.Event()                # the last run of this step, copies included
         self.pending = False
         self.graph: torch.cuda.CUDAGraph | None = None
         self.logits: torch.Tensor | None = None
         self.n_launches = 0
         self.h2d_bytes = total * 4
-        self.d2h_bytes = n_seqs * 4 if sampler is not None else 0
+        self.d2h_bytes = n_out * 4 if sampler is not None else 0
         self.last_slots: list[int] | None = None
         self.last_pos: list[int] | None = None
         self.last_owners = -1                         # the cache's ownership count at the last refresh
+        self.row_stamps: list[list] = []              # of a beam search's step: which rows of pages the staging buffer holds
         # the step is replayed for every length its page tables can address: parts shape their launches for that
         self.kv_capacity = [w * PAGE_TOKENS for w in widths]
 
@@ -167,6 +183,9 @@ class DecodeGraph:
         if self.pending:
             self.done.synchronize()  # the run before must have read the staging buffer
             self.pending = False
+        if self.beams > 1:
+            self._refresh_beams(slots, start_pos, tokens, uniforms)
+            return
         n, h = self.n, self.host_np
         owners = getattr(self.cache, "ownership_changes", None)
         if (self.last_slots == slots and owners is not None and owners == self.last_owners
@@ -188,11 +207,34 @@ class DecodeGraph:
             h[self.uniform_offset:self.uniform_offset + n] = np.asarray(uniforms, dtype=np.float32).view(np.int32)
         self.last_slots, self.last_pos, self.last_owners = list(slots), list(start_pos), owners
 
+    def _refresh_beams(self, slots, start_pos, tokens, scores) -> None:
+        """The same for a beam search's step, whose beams change places and pages at every step: only the rows of pages that
+        the buffer does not hold already are written."""
+        n, h, groups = self.n, self.host_np, self.cache.paged_groups
+        if not self.row_stamps:
+            pieces, _, _ = _pack(self.cache, slots, start_pos, [[t] for t in tokens], list(range(n)), self.widths)
+            np.concatenate(pieces, out=h[:self.shared_offset])
+            self.row_stamps = [[None] * n for _ in groups]
+        else:
+            h[0:n] = tokens
+            h[n:2 * n] = start_pos
+            h[4 * n + 1:5 * n + 1] = h[n:2 * n] + 1
+            h[5 * n + 1:6 * n + 1] = slots
+        for g, stamps, off, w in zip(groups, self.row_stamps, self.table_offsets, self.widths):
+            for i, s in enumerate(slots):
+                stamp = g.stamp(s)
+                if stamps[i] != stamp:
+                    row = g.rows[s]
+                    h[off + i * w: off + i * w + len(row)] = np.maximum(np.asarray(row, dtype=np.int32), 0)
+                    stamps[i] = stamp
+        h[self.shared_offset:self.uniform_offset] = _shared_pages(self.cache, slots, self.beams)
+        h[self.uniform_offset:self.uniform_offset + n] = np.asarray(scores, dtype=np.float32).view(np.int32)
+
     def _launches(self, slots, start_pos):
         """The step as it is issued and as it is recorded: staging buffer in, model, draw, tokens out."""
         self.dev.copy_(self.host, non_blocking=True)
         ctx, rows = _context_over(self.dev, self.sizes, self.table_shapes, self.model.dtype, self.model.device, slots,
-                                  start_pos, [1] * self.n, self.kv_capacity)
+                                  start_pos, [1] * self.n, self.kv_capacity, self.beams)
         if self.fed:
             ctx.tokens = self.tokens_dev  # read by the embedding before this step's draw overwrites it
         logits = self.model.forward(ctx, self.cache, rows)
@@ -223,12 +265,16 @@ class DecodeGraph:
         self.pending = True
         return self.logits
 
-    def sampled(self) -> list[int]:
-        """The tokens drawn by the last run (waits for it)."""
+    def drawn(self) -> torch.Tensor:
+        """What the sampler left in the last run, on the host (waits for it; the next run overwrites it)."""
         if self.pending:
             self.done.synchronize()
             self.pending = False
-        return self.tokens_host.tolist()
+        return self.tokens_host
+
+    def sampled(self) -> list[int]:
+        """The tokens drawn by the last run (waits for it)."""
+        return self.drawn().tolist()
 
 
 class PromptGraph:
@@ -315,7 +361,7 @@ class StepFunction:
         # steps keep theirs in the graph's own memory
         self.workspace = Workspace(model.device) if model.device.type == "cuda" else None
 
-    def _graph_for(self, slots: list[int], start: list[int], sampler=None, variant: int = 0) -> DecodeGraph:
+    def _graph_for(self, slots: list[int], start: list[int], sampler=None, variant: int = 0, beams: int = 1) -> DecodeGraph:
         """The recorded step that fits these sequences: table widths are powers of two of at least 4 pages.
         ``variant`` 0 takes its tokens from the host; 1 and 2 are two copies of the step that takes them from the
         draw before it on the device (two, so that one can be staged while the other runs)."""
@@ -327,17 +373,59 @@ class StepFunction:
             while w < need:
                 w *= 2
             widths.append(w)
-        key = (len(slots), tuple(widths), sampler.launch_key() if sampler is not None else None, variant)
+        key = (len(slots), tuple(widths), sampler.launch_key() if sampler is not None else None, variant, beams)
         g = self._graphs.get(key)
         if g is None:
             drawn = None
-            if sampler is not None:
+            if sampler is not None and not hasattr(sampler, "outputs"):
                 drawn = self._drawn.get(len(slots))
                 if drawn is None:
                     drawn = self._drawn[len(slots)] = torch.empty(len(slots), dtype=torch.int32, device=self.model.device)
             g = self._graphs[key] = DecodeGraph(self.model, cache, len(slots), widths, sampler, tokens_dev=drawn,
-                                                fed=variant != 0)
+                                                fed=variant != 0, beams=beams)
         return g
+
+    def decode_beams(self, inputs: list[SequenceInput], selector, scores: list[float]) -> list[list[tuple[float, int, int]]]:
+        """One decode step of a beam search: the sequences come in groups of ``selector.beams`` that began as one (forks in the cache),
+        ``scores`` are their log probabilities so far.  Returns every group's best continuations (score, beam, token), best first.  As a
+        recorded launch where the step can be one (staging copy, model, selection, copy of the result)."""
+        if self._in_flight:
+            raise StepError("steps launched by decode_ahead have not been collected")
+        n, beams = len(inputs), selector.beams
+        if n == 0 or n % beams or len(scores) != n:
+            raise StepError(f"{n} sequences with {len(scores)} scores do not make groups of {beams} beams")
+        if any(len(s.tokens) != 1 for s in inputs):
+            raise StepError("a decode step takes one token of each sequence")
+        self._validate(inputs)
+        cache = self.cache
+        slots = [s.slot for s in inputs]
+        for i in range(0, n, beams):
+            if len({cache.length(s) for s in slots[i:i + beams]}) > 1:
+                raise StepError(f"the beams in slots {slots[i:i + beams]} are not equally long")
+        cache.reserve([(s, 1) for s in slots])
+        start, tokens = [cache.length(s) for s in slots], [s.tokens[0] for s in inputs]
+        if self.use_graphs and n <= self.max_graph_batch:
+            g = self._graph_for(slots, start, selector, beams=beams)
+            replayed = g.graph is not None
+            g.run(slots, start, tokens, selector.uniforms(scores), before_launch=self.before_launch)
+            self.last_h2d_bytes, self.last_d2h_bytes = g.h2d_bytes, g.d2h_bytes
+            if replayed:
+                self.graph_launches += g.n_launches
+            for s in slots:
+                cache.commit(s, 1)
+            return selector.read(g.drawn())
+        ctx, rows = build_context(self.model.dtype, self.model.device, cache, slots, start, [[t] for t in tokens], list(range(n)),
+                                  self.workspace, beams)
+        logits = self.model.forward(ctx, cache, rows)
+        for s in slots:
+            cache.commit(s, 1)
+        return self.select_beams(logits, selector, scores)
+
+    def select_beams(self, logits: torch.Tensor, selector, scores: list[float]) -> list[list[tuple[float, int, int]]]:
+        """The selection alone, on logits [groups * beams, vocab]."""
+        out = torch.empty(selector.outputs(logits.shape[0]), dtype=torch.int32, device=logits.device)
+        selector.sample_into(logits, torch.tensor(scores, dtype=torch.float32).to(logits.device), out)
+        return selector.read(out.cpu())
 
     def decode_and_sample(self, inputs: list[SequenceInput], sampler, requests: list[int], draws: list[int]):
         """One token per sequence in, one drawn token per sequence out (host integers), as ONE recorded launch:

@@ -57,10 +57,29 @@ def try_decode_attention_with_rope(qkv, out, ctx, page_table, cache, mixer, writ
     if not (ctx.all_decode and ops.attention_decode_rope_supported(qkv.dtype, mixer.n_heads, mixer.n_kv_heads,
                                                                    mixer.head_dim, pos.rotary_dim, pos.pairing)):
         return False
+    if beams_share_attention(ctx, mixer, qkv.dtype):
+        return False
     splits, early = mixer.plan_decode(ctx, cache)
     ops.attention_decode_rope(qkv, out, ctx.kv_lens, page_table, cache.k, cache.v, pos.inverse_frequencies(qkv.device),
                               mixer.n_heads, mixer.n_kv_heads, mixer.head_dim, pos.pairing, mixer.window or 0, splits,
                               write_cache=writes_cache, early_start=early)
+    return True
+
+
+def beams_share_attention(ctx, mixer, dtype) -> bool:
+    """Whether a decode step's attention reads the pages that a group's sequences share once for all of them: a beam search's step of a
+    mixer whose mask is causality and at most a window."""
+    return (getattr(ctx, "beams", 1) > 1 and ctx.all_decode and not (mixer.keep_first or getattr(mixer, "has_terms", False) or getattr(mixer, "chunk", None))
+            and ops.attention_beams_supported(dtype, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim))
+
+
+def try_beam_attention(qkv, out, ctx, page_table, cache, mixer, gate=None) -> bool:
+    if gate is not None or not beams_share_attention(ctx, mixer, qkv.dtype) or qkv.shape[1] % 8 or qkv.data_ptr() & 15:
+        return False
+    parts = ops.attention_beams_parts(ctx.n_seqs // ctx.beams, ctx.beams, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim,
+                                      ctx.capacity(cache.group), qkv.dtype, qkv.device)
+    ops.attention_decode_beams(qkv, qkv.shape[1], out, ctx.kv_lens, page_table, ctx.shared_pages[cache.group], cache.k, cache.v, mixer.n_heads,
+                               mixer.n_kv_heads, mixer.head_dim, mixer.window or 0, parts)
     return True
 
 

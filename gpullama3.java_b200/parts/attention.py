@@ -270,6 +270,8 @@ def attend(shape, qkv: torch.Tensor, out: torch.Tensor, ctx: StepContext, table:
     takes the sizes, else the plain kernel (a step of few tokens cuts their keys into spans so that the GPU has CTAs to
     run).  ``shape`` as for ``plan_decode_attention``, with ``plan_decode``, ``has_terms`` and the terms themselves
     (``slopes``, ``sinks``, ``softcap``) where it has any."""
+    if fast.try_beam_attention(qkv, out, ctx, table, cache, shape, gate):
+        return
     if fast.try_attention(qkv, out, ctx, table, cache, shape, gate):
         return
     terms = dict(chunk=getattr(shape, "chunk", None) or 0, slopes=getattr(shape, "slopes", None), sinks=getattr(shape, "sinks", None),

@@ -47,6 +47,10 @@ class StepContext:
     # once needs no more than max_kv_len; a recorded decode step is replayed while its page tables can address
     # the sequences, so a part that shapes its launch by length (spans of keys) shapes it for this number.
     kv_capacity: list[int] = field(default_factory=list)
+    # a decode step of a beam search: sequences come in groups of ``beams`` that began as one, and per paged cache group
+    # ``shared_pages`` [n_seqs / beams] counts the first pages that are the same in a group's rows of the page table
+    beams: int = 1
+    shared_pages: list[torch.Tensor] | None = None
     extras: dict = field(default_factory=dict)  # scratch a part may keep for the duration of a step
     workspace: object = None         # where intermediate tensors of this pass come from (None: the allocator)
 

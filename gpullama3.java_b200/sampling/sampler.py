@@ -89,3 +89,36 @@ class Sampler:
             ops.argmax_rows(logits, out)
         else:
             ops.sample_rows(logits, uniforms, out, self.params.temperature, self.params.top_p)
+
+
+class BeamSelector:
+    """The selection of a beam search as a step function records it: of every group of ``beams`` sequences the ``keep`` best
+    continuations, by the beams' scores (log probabilities so far) and the step's logits."""
+
+    def __init__(self, beams: int, keep: int):
+        if not ops.beam_select_takes(beams, keep):
+            raise ValueError(f"{beams} beams with {keep} continuations: at most 1,024 and {ops.BEAM_MAX_KEEP}")
+        self.beams, self.keep = beams, keep
+
+    def launch_key(self):
+        return ("beams", self.beams, self.keep)
+
+    def outputs(self, n_seqs: int) -> int:
+        """32-bit words a step leaves: scores, beams and tokens of every group's continuations."""
+        return 3 * (n_seqs // self.beams) * self.keep
+
+    def uniforms(self, scores, draws=None) -> list[float]:
+        """The host-side input of one step: the beams' scores."""
+        return list(scores)
+
+    def sample_into(self, logits: torch.Tensor, scores: torch.Tensor, out: torch.Tensor) -> None:
+        """Scores, beams and tokens [groups, keep] one after the other into ``out`` (int32; the scores' bits)."""
+        G = logits.shape[0] // self.beams
+        s, b, t = (x.view(G, self.keep) for x in out.view(3, G * self.keep))
+        ops.beam_select(logits, scores.view(G, self.beams), s.view(torch.float32), b, t)
+
+    def read(self, words) -> list[list[tuple[float, int, int]]]:
+        """Per group the continuations (score, beam, token), best first, from what ``sample_into`` left (on the host)."""
+        words = torch.as_tensor(words, dtype=torch.int32).view(3, -1, self.keep)
+        scores, beams, tokens = words[0].view(torch.float32).tolist(), words[1].tolist(), words[2].tolist()
+        return [[(s, b, t) for s, b, t in zip(*rows) if t >= 0] for rows in zip(scores, beams, tokens)]
