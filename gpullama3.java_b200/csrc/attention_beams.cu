@@ -7,8 +7,10 @@
 // tile: at 8 beams of 32 heads on 8 that is 32 rows, and an eighth of the bytes that as many separate sequences read.
 //
 // The work is cut by pages.  The pages of one segment belong together: the shared pages of a group, then the pages that each
-// of its sequences has for itself, group after group.  All segments' pages in this order are numbered, and of every kv head each of
-// gridDim.x CTAs takes as many consecutive ones, whatever they belong to, so groups of unequal length share the GPU evenly.
+// of its sequences has for itself, group after group.  All segments in this order make one line, on which a page is 1 long and a segment with
+// pages kSegmentCost longer (what it costs to begin and leave one); of every kv head each of gridDim.x CTAs takes the pages of an equal
+// stretch, whatever they belong to, so groups of unequal length share the GPU evenly.  The line is laid out by each CTA for itself, or once for all
+// layers of a step by attention_beams_plan.
 // A CTA keeps the running maximum m, sum l and output o of a segment's rows in registers and leaves them, unnormalised, in
 // scratch at the segment's end or its own; a second kernel joins what the CTAs left of a row, in a fixed order.  CTA c's piece of
 // segment s is number c + s (along the pages either grows, so no two pieces have one number).
@@ -33,37 +35,154 @@ struct BeamAttnArgs {
     const void* v_pool;
     float* part_o;                      // [kv_head][piece][row][D]
     float* part_ml;                     // [kv_head][piece][row][2]
-    int* plan;                          // [0] pages of a CTA, [1 + s] first page number of segment s, of which the last is the end
+    int* plan;                          // the segments, as many ints as plan_ints
+    int given;                          // whether they are there already
+    unsigned per_magic;                 // 2^32 / (sub_beams + 1), rounded up
     long long q_row_stride;
-    int table_stride, n_seqs, n_groups, beams, sub_beams, n_sub, n_heads, n_kv_heads, window;
+    int table_stride, n_seqs, n_groups, beams, sub_beams, n_sub, n_parts, n_segments, n_heads, n_kv_heads, window;
 };
 
 __device__ __forceinline__ int first_key(int kv_len, int window) { return window > 0 ? max(0, kv_len - window) : 0; }
 
-// Segments: part p of n_groups * n_sub (n_sub parts of up to sub_beams sequences to a group) has its shared pages as segment p * (sub_beams + 1),
-// its sequences' own as the next ones.
+// Segments: part p of n_parts = n_groups * n_sub (n_sub parts of up to sub_beams sequences to a group) has its shared pages as segment
+// p * (sub_beams + 1), its sequences' own as the next ones.
 __device__ __forceinline__ int part_first_row(const BeamAttnArgs& a, int p) { return (p / a.n_sub) * a.beams + (p % a.n_sub) * a.sub_beams; }
 __device__ __forceinline__ int part_rows(const BeamAttnArgs& a, int p) { return min(a.sub_beams, a.beams - (p % a.n_sub) * a.sub_beams); }
-// the shared pages [lo, hi) that some sequence of the part reads; hi bounds the sequences' own pages from below
-__device__ __forceinline__ void shared_range(const BeamAttnArgs& a, int p, int& lo, int& hi) {
-    const int r0 = part_first_row(a, p), n = part_rows(a, p);
-    hi = min(max(a.shared_pages[p / a.n_sub], 0), a.table_stride);
-    int first = 0x7fffffff;
-    for (int i = 0; i < n; ++i) {
-        const int len = max(a.kv_lens[r0 + i], 0);
-        hi = min(hi, len / kPageTokens);
-        first = min(first, first_key(len, a.window));
+
+__device__ __forceinline__ int part_of_segment(const BeamAttnArgs& a, int s) { return (int)__umulhi((unsigned)s, a.per_magic); }   // (s below 2^16)
+
+constexpr int kSegmentCost = 1;
+struct Segment {
+    int pages;          // pages before it
+    int at;             // where it begins on the line
+    int lo;             // its first page's place in the page table
+    int row;            // the sequence whose row of the table that is
+};
+// In shared memory: [n_segments + 1] of these, the last one's `pages` and `at` the ends; then the sequences' lengths (as far as they are
+// needed) and the parts' shared pages.
+static int plan_ints(const BeamAttnArgs& a) { return 4 * (a.n_segments + 1) + a.n_seqs + 2 * a.n_parts; }
+// the length of a CTA's stretch
+__device__ __forceinline__ int stretch_of(int line, int ctas) { return max(1, (line + ctas - 1) / ctas); }
+
+// Lays the line out.  By all threads of a CTA.  `tmp`: two ints for each warp.
+template <int THREADS>
+__device__ __forceinline__ void make_plan(const BeamAttnArgs& a, Segment* seg, int* lens, int* tmp) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int* range = lens + a.n_seqs;
+    for (int i = tid; i < a.n_seqs; i += THREADS) lens[i] = max(a.kv_lens[i], 0);
+    for (int p = tid; p < a.n_parts; p += THREADS) range[2 * p + 1] = min(max(a.shared_pages[a.n_sub == 1 ? p : p / a.n_sub], 0), a.table_stride);
+    __syncthreads();
+    // shared pages: those that some sequence of the part reads, as far as they are full for all
+    for (int p = tid; p < a.n_parts; p += THREADS) {
+        const int r0 = part_first_row(a, p), n = part_rows(a, p);
+        int shortest = lens[r0];
+        for (int i = 1; i < n; ++i) shortest = min(shortest, lens[r0 + i]);
+        const int hi = min(range[2 * p + 1], shortest / kPageTokens);
+        range[2 * p] = min(first_key(shortest, a.window) / kPageTokens, hi);
+        range[2 * p + 1] = hi;
     }
-    lo = min(first / kPageTokens, hi);
+    __syncthreads();
+    // a thread's consecutive segments: their pages are counted, then added up in order
+    const int each = (a.n_segments + THREADS - 1) / THREADS, s0 = tid * each, s1 = min(a.n_segments, s0 + each);
+    int pages = 0, line = 0;
+    for (int s = s0; s < s1; ++s) {
+        const int p = part_of_segment(a, s), i = s - p * (a.sub_beams + 1), r0 = part_first_row(a, p);
+        int lo = range[2 * p], hi = range[2 * p + 1], row = r0;
+        if (i > 0) {
+            lo = hi;
+            if (i <= part_rows(a, p)) {
+                row = r0 + i - 1;
+                const int len = lens[row];
+                hi = min((len + kPageTokens - 1) / kPageTokens, a.table_stride);
+                lo = min(max(lo, first_key(len, a.window) / kPageTokens), hi);
+            }
+        }
+        seg[s] = Segment{hi - lo, 0, lo, row};
+        pages += hi - lo;
+        line += hi > lo ? hi - lo + kSegmentCost : 0;
+    }
+    int pages_to = pages, line_to = line;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, pages_to, o), w = __shfl_up_sync(0xffffffffu, line_to, o);
+        if (lane >= o) { pages_to += v; line_to += w; }
+    }
+    if (lane == 31) { tmp[2 * warp] = pages_to; tmp[2 * warp + 1] = line_to; }
+    __syncthreads();
+    int pages_before = pages_to - pages, line_before = line_to - line;
+    for (int w = 0; w < warp; ++w) { pages_before += tmp[2 * w]; line_before += tmp[2 * w + 1]; }
+    for (int s = s0; s < s1; ++s) {
+        const int n = seg[s].pages;
+        seg[s].pages = pages_before;
+        seg[s].at = line_before;
+        pages_before += n;
+        line_before += n > 0 ? n + kSegmentCost : 0;
+    }
+    if (tid == THREADS - 1) seg[a.n_segments] = Segment{pages_before, line_before, 0, 0};
+    __syncthreads();
 }
-__device__ __forceinline__ void own_range(const BeamAttnArgs& a, int row, int shared_hi, int& lo, int& hi) {
-    const int len = max(a.kv_lens[row], 0);
-    hi = min((len + kPageTokens - 1) / kPageTokens, a.table_stride);
-    lo = min(max(shared_hi, first_key(len, a.window) / kPageTokens), hi);
+
+// The same for a CTA that is given the plan, and for one that is not (CTA 0, 0 of those leaves it for the kernel that joins the pieces).
+template <int THREADS>
+__device__ __forceinline__ void take_plan(const BeamAttnArgs& a, Segment* seg, int* lens, int* tmp) {
+    if (a.given) {
+        for (int i = threadIdx.x; i <= a.n_segments; i += THREADS) reinterpret_cast<int4*>(seg)[i] = reinterpret_cast<const int4*>(a.plan)[i];
+        for (int i = threadIdx.x; i < a.n_seqs; i += THREADS) lens[i] = max(a.kv_lens[i], 0);
+        __syncthreads();
+        return;
+    }
+    make_plan<THREADS>(a, seg, lens, tmp);
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int i = threadIdx.x; i <= a.n_segments; i += THREADS) reinterpret_cast<int4*>(a.plan)[i] = reinterpret_cast<const int4*>(seg)[i];
+}
+
+__global__ void __launch_bounds__(256) attention_beams_plan_kernel(const __grid_constant__ BeamAttnArgs a) {
+    extern __shared__ __align__(16) int plan_smem[];
+    __shared__ int tmp[16];
+    Segment* seg = reinterpret_cast<Segment*>(plan_smem);
+    pdl_launch_dependents();
+    pdl_wait();
+    make_plan<256>(a, seg, plan_smem + 4 * (a.n_segments + 1), tmp);
+    for (int i = threadIdx.x; i <= a.n_segments; i += 256) reinterpret_cast<int4*>(a.plan)[i] = reinterpret_cast<const int4*>(seg)[i];
+}
+
+// the last of the segments that begin at or before `x` on the line (by_pages: before whose end page number x lies, and which is not empty)
+template <bool BY_PAGES>
+__device__ __forceinline__ int segment_at(const BeamAttnArgs& a, const Segment* seg, int x) {
+    int lo = 0, hi = a.n_segments - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((BY_PAGES ? seg[mid].pages : seg[mid].at) <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+// the number of pages that begin before place x of the line
+__device__ __forceinline__ int pages_before(const BeamAttnArgs& a, const Segment* seg, int x) {
+    if (x >= seg[a.n_segments].at) return seg[a.n_segments].pages;
+    const int s = segment_at<false>(a, seg, x);
+    return seg[s].pages + min(max(x - seg[s].at - kSegmentCost, 0), seg[s + 1].pages - seg[s].pages);
+}
+
+// A page of the work: where it lies, whose it is, its first position, and how many of its keys there are.
+struct Unit {
+    int page, segment, position, keys;
+};
+__device__ __forceinline__ Unit unit_of(const BeamAttnArgs& a, const Segment* seg, const int* lens, int u) {
+    Unit x;
+    x.segment = segment_at<true>(a, seg, u);
+    const Segment s = seg[x.segment];
+    const int index = s.lo + u - s.pages;
+    x.page = a.page_table[(size_t)s.row * a.table_stride + index];
+    x.position = index * kPageTokens;
+    x.keys = min(kPageTokens, lens[s.row] - x.position);
+    return x;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t to, const void* from, int bytes) {      // the rest of the 16 is filled with zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -87,83 +206,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// A page of the work: whose it is, where, and how much of it holds keys.
-struct Unit {
-    int page, segment, position, keys;
-};
-
-// The plan, by all threads of a CTA: seg_s[s] = number of pages before segment s, seg_s[n_segments] = all.  `tmp`: an int for each warp.
-template <int THREADS>
-__device__ __forceinline__ void make_plan(const BeamAttnArgs& a, int n_segments, int* seg_s, int* tmp) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per_part = a.sub_beams + 1;
-    // a thread's consecutive segments, their pages first counted, then added up in order
-    const int each = (n_segments + THREADS - 1) / THREADS, s0 = tid * each, s1 = min(n_segments, s0 + each);
-    int total = 0;
-    for (int s = s0; s < s1; ++s) {
-        const int p = s / per_part, i = s % per_part;
-        int lo, hi, n = 0;
-        shared_range(a, p, lo, hi);
-        if (i == 0) n = hi - lo;
-        else if (i <= part_rows(a, p)) {
-            own_range(a, part_first_row(a, p) + i - 1, hi, lo, hi);
-            n = hi - lo;
-        }
-        seg_s[s] = n;
-        total += n;
-    }
-    int incl = total;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-    }
-    if (lane == 31) tmp[warp] = incl;
-    __syncthreads();
-    int before = incl - total;
-    for (int w = 0; w < warp; ++w) before += tmp[w];
-    for (int s = s0; s < s1; ++s) {
-        const int n = seg_s[s];
-        seg_s[s] = before;
-        before += n;
-    }
-    if (tid == THREADS - 1) seg_s[n_segments] = before;
-    __syncthreads();
-}
-
-// the last segment that starts at or before page number u (and is not empty, u being one of its pages)
-__device__ __forceinline__ int segment_of(const int* seg_s, int n_segments, int u) {
-    int lo = 0, hi = n_segments - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (seg_s[mid] <= u) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-}
-__device__ __forceinline__ Unit unit_of(const BeamAttnArgs& a, const int* seg_s, int n_segments, int u) {
-    Unit x;
-    x.segment = segment_of(seg_s, n_segments, u);
-    const int per_part = a.sub_beams + 1, p = x.segment / per_part, i = x.segment % per_part;
-    int lo, hi;
-    shared_range(a, p, lo, hi);
-    const int r0 = part_first_row(a, p), row = i == 0 ? r0 : r0 + i - 1;
-    if (i > 0) own_range(a, row, hi, lo, hi);
-    const int index = lo + u - seg_s[x.segment];
-    x.page = a.page_table[(size_t)row * a.table_stride + index];
-    x.position = index * kPageTokens;
-    x.keys = i == 0 ? kPageTokens : min(kPageTokens, a.kv_lens[row] - x.position);
-    return x;
-}
-
-// bfloat16, on mma.sync.  A warp owns a tile of 16 rows and, where there are fewer than four tiles, a part of each page's keys.
+// bfloat16, on mma.sync.  A warp owns a tile of 16 rows and, where there are fewer than four tiles, a part of each page's keys.  Rows of shared
+// memory are such that the eight rows of an ldmatrix block meet no bank twice: 128 or 256 bytes with their 16-byte pieces exchanged
+// by the row's last three bits, others with 16 bytes between them.
 template <int D>
 struct BeamTile {
-    static constexpr int kPitchK = 2 * D + 16, kPitchV = 2 * kPageTokens + 16;  // bytes; an odd number of 16: ldmatrix meets no bank twice
+    static constexpr bool kExchange = D % 64 == 0;
+    static constexpr int kPitchK = kExchange ? 2 * D : 2 * D + 16, kPitchV = 2 * kPageTokens;       // bytes
     static constexpr int kStage = kPageTokens * kPitchK + D * kPitchV;
-    static constexpr int kStages = D <= 64 ? 3 : 2;
-    static constexpr int kQ = kBaRows * kPitchK;
-    static constexpr int kJoin = 2 * 16 * (D + 4) * 4;                          // two tiles' o, m, l
-    static constexpr int kBytes = kStages * kStage + kQ + kJoin;
+    static __device__ __forceinline__ uint32_t k_piece(int row, int c) { return row * kPitchK + ((kExchange ? c ^ (row & 7) : c) << 4); }
+    static __device__ __forceinline__ uint32_t v_piece(int row, int c) { return row * kPitchV + ((c ^ (row & 7)) << 4); }
 };
 
 template <int D>
@@ -180,74 +232,87 @@ struct RowState {
     }
 };
 
-// One page's keys [part * 64 / KP, ...) for the tile whose query fragments' rows start at q_addr (this lane's ldmatrix address).
-template <int D, int KP>
-__device__ __forceinline__ void attend_page(RowState<D>& st, uint32_t q_addr, uint32_t k_base, uint32_t v_base, int part, int lane, float scale_log2,
-                                            bool masked, int position, const int (&row_lo)[2], int row_end) {
-    constexpr int NK = kPageTokens / KP, NT = NK / 8;
+// NK keys of a page, from its key `first` on, for the tile whose query fragments are qa.  The maximum that exponentials are relative to follows the
+// rows' own only when they have outgrown it by 2^8: until then nothing is rescaled, and probabilities of up to 2^8 keep their bits as well.
+template <int D, int NK>
+__device__ __forceinline__ void attend_keys(RowState<D>& st, const uint32_t (&qa)[D / 16][4], uint32_t k_base, uint32_t v_base, int first, int lane,
+                                            float scale_log2, bool masked, int position, const int (&row_lo)[2], int row_end) {
+    constexpr int NT = NK / 8;
     using T = BeamTile<D>;
-    const int t = lane & 3;
     float s[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[i][c] = 0.f;
     // ldmatrix: lanes 0-7, 8-15, 16-23, 24-31 give the rows of the four 8 x 8 blocks (keys 0-7 and 8-15 by 8 dimensions and the next 8)
-    const uint32_t k_lane = k_base + (uint32_t)((part * NK + (lane & 7) + (lane >> 4) * 8) * T::kPitchK + ((lane >> 3) & 1) * 16);
+    const int low = lane & 7, half = (lane >> 3) & 1, row = low + (lane >> 4) * 8;
+    const uint32_t k_row = k_base + (uint32_t)((first + row) * T::kPitchK);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t qa[4];
-        ldmatrix4(qa, q_addr + ks * 32);
+        const int c = ks * 2 + half;
+        const uint32_t piece = (uint32_t)((T::kExchange ? c ^ low : c) << 4);
 #pragma unroll
         for (int i = 0; i < NT; i += 2) {
             uint32_t kb[4];
-            ldmatrix4(kb, k_lane + (uint32_t)(i * 8 * T::kPitchK + ks * 32));
-            mma_bf16(s[i], qa, kb[0], kb[1]);
-            mma_bf16(s[i + 1], qa, kb[2], kb[3]);
+            ldmatrix4(kb, k_row + piece + (uint32_t)(i * 8 * T::kPitchK));
+            mma_bf16(s[i], qa[ks], kb[0], kb[1]);
+            mma_bf16(s[i + 1], qa[ks], kb[2], kb[3]);
         }
+    }
+    if (masked) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int key = position + first + 8 * i + 2 * (lane & 3) + (c & 1);
+                if (key < row_lo[c >> 1] || key >= row_end) s[i][c] = -INFINITY;
+            }
     }
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            s[i][c] *= scale_log2;
-            if (masked) {
-                const int key = position + part * NK + 8 * i + 2 * t + (c & 1);
-                if (key < row_lo[c >> 1] || key >= row_end) s[i][c] = -INFINITY;
-            }
-            top[c >> 1] = fmaxf(top[c >> 1], s[i][c]);
-        }
+        for (int c = 0; c < 4; ++c) top[c >> 1] = fmaxf(top[c >> 1], s[i][c]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        const float m = fmaxf(st.m[h], top[h]);
-        const float base = m == -INFINITY ? 0.f : m;        // (a row that has seen nothing yet: its probabilities are 0)
-        const float keep = exp2_fast(st.m[h] - base);
-        st.m[h] = m;
-        st.l[h] *= keep;
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)) * scale_log2;
+    }
+    if (__any_sync(0xffffffffu, top[0] > st.m[0] + 8.f || top[1] > st.m[1] + 8.f)) {
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) { st.o[j][2 * h] *= keep; st.o[j][2 * h + 1] *= keep; }
+        for (int h = 0; h < 2; ++h) {
+            const float m = fmaxf(st.m[h], top[h]), keep = m == -INFINITY ? 1.f : exp2_fast(st.m[h] - m);
+            st.m[h] = m;
+            st.l[h] *= keep;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) { st.o[j][2 * h] *= keep; st.o[j][2 * h + 1] *= keep; }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float base = st.m[h] == -INFINITY ? 0.f : st.m[h];        // (a row that has seen nothing yet: its probabilities are 0)
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float p = exp2_fast(s[i][2 * h + e] - base);
-                st.l[h] += p;
+                const float p = exp2_fast(fmaf(s[i][2 * h + e], scale_log2, -base));
+                sum += p;
                 s[i][2 * h + e] = p;
             }
+        st.l[h] += sum;
     }
-    const uint32_t v_lane = v_base + (uint32_t)(((lane & 7) + (lane >> 4) * 8) * T::kPitchV + (part * NK + ((lane >> 3) & 1) * 8) * 2);
+    const uint32_t v_row = v_base + (uint32_t)(row * T::kPitchV);
 #pragma unroll
     for (int kk = 0; kk < NK / 16; ++kk) {
         // probabilities are rounded to bfloat16 for the tensor cores, as the values are stored; their sum l is not
         const uint32_t pa[4] = {pack2(s[2 * kk][0], s[2 * kk][1]), pack2(s[2 * kk][2], s[2 * kk][3]),
                                 pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+        const uint32_t piece = (uint32_t)((((first >> 3) + kk * 2 + half) ^ low) << 4);
 #pragma unroll
         for (int j = 0; j < D / 8; j += 2) {
             uint32_t vb[4];
-            ldmatrix4(vb, v_lane + (uint32_t)(j * 8 * T::kPitchV + kk * 32));
+            ldmatrix4(vb, v_row + piece + (uint32_t)(j * 8 * T::kPitchV));
             mma_bf16(st.o[j], pa, vb[0], vb[1]);
             mma_bf16(st.o[j + 1], pa, vb[2], vb[3]);
         }
@@ -307,127 +372,138 @@ __device__ __forceinline__ void leave_tile(RowState<D>& st, float* join, int par
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __grid_constant__ BeamAttnArgs a, int n_segments) {
+// STAGES pages are in shared memory or on their way there.  A piece's parts are joined in the stage that was read last.
+template <int D, int STAGES>
+__global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __grid_constant__ BeamAttnArgs a) {
     using T = BeamTile<D>;
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int tmp[kBaThreads / 32];
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int tmp[kBaThreads / 16];
     __shared__ Unit ring[kBaRing];
-    unsigned char* q_s = smem + T::kStages * T::kStage;
-    float* join = reinterpret_cast<float*>(q_s + T::kQ);
-    int* seg_s = reinterpret_cast<int*>(q_s + T::kQ + T::kJoin);
+    unsigned char* q_s = smem + STAGES * T::kStage;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int kvh = blockIdx.y, rep = a.n_heads / a.n_kv_heads, per_part = a.sub_beams + 1;
-    pdl_launch_dependents();
+    const int kvh = blockIdx.y, rep = a.n_heads / a.n_kv_heads;
+    Segment* seg = reinterpret_cast<Segment*>(q_s + a.sub_beams * rep * T::kPitchK);
+    int* lens = reinterpret_cast<int*>(seg + a.n_segments + 1);
     pdl_wait();
-    make_plan<kBaThreads>(a, n_segments, seg_s, tmp);
-    const int all = seg_s[n_segments], per = max(1, (all + (int)gridDim.x - 1) / (int)gridDim.x);
-    if (blockIdx.x == 0 && kvh == 0) {      // for the kernel that joins the pieces
-        for (int s = tid; s <= n_segments; s += kBaThreads) a.plan[1 + s] = seg_s[s];
-        if (tid == 0) a.plan[0] = per;
-    }
-    const int u0 = blockIdx.x * per, u1 = min(all, u0 + per);
+    // (only now: the kernel that joins the pieces may read a given plan as soon as it starts)
+    pdl_launch_dependents();
+    take_plan<kBaThreads>(a, seg, lens, tmp);
+    const int per = stretch_of(seg[a.n_segments].at, gridDim.x);
+    const int u0 = pages_before(a, seg, blockIdx.x * per), u1 = pages_before(a, seg, (blockIdx.x + 1) * per);
     if (u0 >= u1) return;
 
     const size_t page_elements = (size_t)a.n_kv_heads * kPageTokens * D, head_off = (size_t)kvh * kPageTokens * D;
     const uint32_t stage0 = (uint32_t)__cvta_generic_to_shared(smem), q_base = (uint32_t)__cvta_generic_to_shared(q_s);
+    constexpr int CK = D / 8, CV = kPageTokens / 8;        // 16-byte pieces of a row
     auto know = [&](int u) {        // pages u .. u + 31 into the ring
-        if (tid < kBaKnown && u + tid < u1) ring[(u + tid - u0) % kBaRing] = unit_of(a, seg_s, n_segments, u + tid);
+        if (tid < kBaKnown && u + tid < u1) ring[(u + tid - u0) % kBaRing] = unit_of(a, seg, lens, u + tid);
     };
     auto issue = [&](int u) {
         if (u < u1) {
             const Unit x = ring[(u - u0) % kBaRing];
-            const uint32_t ks = stage0 + (uint32_t)(((u - u0) % T::kStages) * T::kStage), vs = ks + kPageTokens * T::kPitchK;
+            const uint32_t ks = stage0 + (uint32_t)(((u - u0) % STAGES) * T::kStage), vs = ks + kPageTokens * T::kPitchK;
             const __nv_bfloat16* k = (const __nv_bfloat16*)a.k_pool + (size_t)x.page * page_elements + head_off;
             const __nv_bfloat16* v = (const __nv_bfloat16*)a.v_pool + (size_t)x.page * page_elements + head_off;
-            constexpr int CK = D / 8, CV = kPageTokens / 8;        // 16-byte pieces of a row
+            constexpr int RK = kBaThreads / CK, RV = kBaThreads / CV;
+            if (x.keys == kPageTokens && kBaThreads % CK == 0 && RK % 8 == 0) {   // a thread's pieces lie whole rows apart, at one place in them
+                const uint32_t kt = ks + T::k_piece(tid / CK, tid % CK), vt = vs + T::v_piece(tid / CV, tid % CV);
+                k += tid * 8;
+                v += tid * 8;
 #pragma unroll
-            for (int i = tid; i < kPageTokens * CK; i += kBaThreads) {
-                const int row = i / CK, c = i % CK;
-                cp_async16(ks + row * T::kPitchK + c * 16, k + (size_t)row * D + c * 8, row < x.keys ? 16 : 0);
-            }
-            // (values of positions past the sequence's end are read as zeros: a probability of 0 times what is not finite is not 0)
+                for (int i = 0; i < kPageTokens / RK; ++i) cp_async16(kt + i * RK * T::kPitchK, k + i * kBaThreads * 8);
 #pragma unroll
-            for (int i = tid; i < D * CV; i += kBaThreads) {
-                const int row = i / CV, c = i % CV;
-                cp_async16(vs + row * T::kPitchV + c * 16, v + (size_t)row * kPageTokens + c * 8, min(16, max(0, 2 * (x.keys - 8 * c))));
+                for (int i = 0; i < D / RV; ++i) cp_async16(vt + i * RV * T::kPitchV, v + i * kBaThreads * 8);
+            } else {
+                for (int i = tid; i < kPageTokens * CK; i += kBaThreads)
+                    cp_async16(ks + T::k_piece(i / CK, i % CK), k + (size_t)i * 8, i / CK < x.keys ? 16 : 0);
+                // (values of positions past the sequence's end are read as zeros: a probability of 0 times what is not finite is not 0)
+                for (int i = tid; i < D * CV; i += kBaThreads)
+                    cp_async16(vs + T::v_piece(i / CV, i % CV), v + (size_t)i * 8, min(16, max(0, 2 * (x.keys - 8 * (i % CV)))));
             }
         }
         cp_async_commit();
     };
+    auto ask_queries = [&](int p) {     // of all rows of part p
+        const int r0 = part_first_row(a, p);
+        for (int c = tid; c < part_rows(a, p) * rep * CK; c += kBaThreads) {
+            const int row = c / CK, at = c % CK;
+            cp_async16(q_base + T::k_piece(row, at), (const __nv_bfloat16*)a.q + (size_t)(r0 + row / rep) * a.q_row_stride
+                                                         + (size_t)(kvh * rep + row % rep) * D + at * 8);
+        }
+    };
     know(u0);
     __syncthreads();
+    int part_of = part_of_segment(a, ring[0].segment);
+    ask_queries(part_of);               // (they arrive with the first page)
 #pragma unroll
-    for (int i = 0; i < T::kStages - 1; ++i) issue(u0 + i);
+    for (int i = 0; i < STAGES - 1; ++i) issue(u0 + i);
 
     const float scale_log2 = 1.4426950408889634f / sqrtf((float)D);
     RowState<D> st;
-    int segment = -1, part_of = -1, parts = 1, part = 0, tile = warp, rows = 0, q_row = 0, lo_max = 0, row_end = 0, row_lo[2] = {0, 0};
-    auto leave = [&]() {
-        const size_t piece = (size_t)kvh * (gridDim.x + n_segments) + blockIdx.x + segment;
-        leave_tile<D>(st, join, parts, part, tile, lane, rows, a.part_o + piece * kBaRows * D, a.part_ml + piece * kBaRows * 2);
+    uint32_t qa[D / 16][4];
+    int segment = -1, parts = 1, part = 0, tile = warp, rows = 0, lo_max = 0, row_end = 0, row_lo[2] = {0, 0};
+    auto leave = [&](int u) {           // behind page u - 1, with its stage to join in
+        const size_t piece = (size_t)kvh * (gridDim.x + a.n_segments) + blockIdx.x + segment;
+        leave_tile<D>(st, reinterpret_cast<float*>(smem + ((u - 1 - u0) % STAGES) * T::kStage), parts, part, tile, lane, rows,
+                      a.part_o + piece * kBaRows * D, a.part_ml + piece * kBaRows * 2);
     };
     for (int u = u0; u < u1; ++u) {
-        cp_async_wait<T::kStages - 2>();
+        cp_async_wait<STAGES - 2>();
         __syncthreads();
-        const int ahead = u + T::kStages - 1;
-        if (ahead < u1 && ahead > u0 && (ahead - u0) % kBaKnown == 0) {
+        const Unit x = ring[(u - u0) % kBaRing];
+        if (x.segment != segment) {
+            if (segment >= 0) {
+                leave(u);
+                __syncthreads();
+            }
+            segment = x.segment;
+            st.clear();
+            const int p = part_of_segment(a, segment), i = segment - p * (a.sub_beams + 1), r0 = part_first_row(a, p), n = part_rows(a, p);
+            if (p != part_of) {
+                part_of = p;
+                ask_queries(p);
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncthreads();
+            }
+            rows = i == 0 ? n * rep : rep;
+            parts = rows <= 16 ? 4 : rows <= 32 ? 2 : 1;
+            tile = warp % (4 / parts);
+            part = warp / (4 / parts);
+            row_end = i == 0 ? 0x7fffffff : lens[r0 + i - 1];
+            lo_max = 0;
+            if (a.window > 0) {
+                for (int b = 0; b < n; ++b) lo_max = max(lo_max, first_key(lens[r0 + b], a.window));
+                if (i > 0) lo_max = first_key(row_end, a.window);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    row_lo[h] = i > 0 ? lo_max : first_key(lens[r0 + min(tile * 16 + (lane >> 2) + 8 * h, rows - 1) / rep], a.window);
+            }
+            // (rows behind the last one are its copies, and nothing of them is stored)
+            const int row = min(tile * 16 + (lane & 15), rows - 1) + (i == 0 ? 0 : (i - 1) * rep);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) ldmatrix4(qa[ks], q_base + T::k_piece(row, ks * 2 + (lane >> 4)));
+        }
+        const int ahead = u + STAGES - 1;
+        if (ahead < u1 && (ahead - u0) % kBaKnown == 0) {
             know(ahead);
             __syncthreads();
         }
         issue(ahead);
-        const Unit x = ring[(u - u0) % kBaRing];
-        if (x.segment != segment) {
-            if (segment >= 0) leave();
-            segment = x.segment;
-            st.clear();
-            const int p = segment / per_part, i = segment % per_part;
-            const int r0 = part_first_row(a, p), n = part_rows(a, p);
-            if (p != part_of) {         // the queries of all of the part's rows
-                __syncthreads();
-                part_of = p;
-                constexpr int CQ = D / 8;
-                for (int c = tid; c < n * rep * CQ; c += kBaThreads) {
-                    const int row = c / CQ, at = c % CQ;
-                    const __nv_bfloat16* from = (const __nv_bfloat16*)a.q + (size_t)(r0 + row / rep) * a.q_row_stride
-                                                + (size_t)(kvh * rep + row % rep) * D + at * 8;
-                    *reinterpret_cast<uint4*>(q_s + row * T::kPitchK + at * 16) = *reinterpret_cast<const uint4*>(from);
-                }
-                __syncthreads();
-            }
-            rows = i == 0 ? n * rep : rep;
-            q_row = i == 0 ? 0 : (i - 1) * rep;
-            const int tiles = (rows + 15) / 16;
-            parts = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;
-            tile = warp % (4 / parts);
-            part = warp / (4 / parts);
-            lo_max = 0;
-            if (i == 0) {
-                for (int b = 0; b < n; ++b) lo_max = max(lo_max, first_key(a.kv_lens[r0 + b], a.window));
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = min(tile * 16 + (lane >> 2) + 8 * h, rows - 1);
-                    row_lo[h] = first_key(a.kv_lens[r0 + r / rep], a.window);
-                }
-                row_end = 0x7fffffff;
-            } else {
-                row_end = a.kv_lens[r0 + i - 1];
-                lo_max = row_lo[0] = row_lo[1] = first_key(row_end, a.window);
-            }
-        }
         if (tile * 16 < rows) {
-            // (rows behind the last one are its copies, and nothing of them is stored)
-            const int row = min(tile * 16 + (lane & 15), rows - 1) + q_row;
-            const uint32_t q_addr = q_base + (uint32_t)(row * T::kPitchK + (lane >> 4) * 16);
-            const uint32_t ks = stage0 + (uint32_t)(((u - u0) % T::kStages) * T::kStage), vs = ks + kPageTokens * T::kPitchK;
+            const uint32_t ks = stage0 + (uint32_t)(((u - u0) % STAGES) * T::kStage), vs = ks + kPageTokens * T::kPitchK;
             const bool masked = x.keys < kPageTokens || x.position < lo_max;
-            if (parts == 4) attend_page<D, 4>(st, q_addr, ks, vs, part, lane, scale_log2, masked, x.position, row_lo, row_end);
-            else if (parts == 2) attend_page<D, 2>(st, q_addr, ks, vs, part, lane, scale_log2, masked, x.position, row_lo, row_end);
-            else attend_page<D, 1>(st, q_addr, ks, vs, part, lane, scale_log2, masked, x.position, row_lo, row_end);
+            if (parts == 4) {
+                attend_keys<D, 16>(st, qa, ks, vs, part * 16, lane, scale_log2, masked, x.position, row_lo, row_end);
+            } else {
+#pragma unroll 1
+                for (int first = part * 32; first < kPageTokens; first += parts * 32)
+                    attend_keys<D, 32>(st, qa, ks, vs, first, lane, scale_log2, masked, x.position, row_lo, row_end);
+            }
         }
     }
-    leave();
     cp_async_wait<0>();
+    leave(u1);
 }
 
 // float32, on multiply-adds.  Scores: a thread holds one key's dimensions in registers and takes every fourth row's query from shared memory
@@ -446,34 +522,31 @@ struct BeamTileF32 {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const __grid_constant__ BeamAttnArgs a, int n_segments) {
+__global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const __grid_constant__ BeamAttnArgs a) {
     using T = BeamTileF32<D>;
     extern __shared__ __align__(16) float smem_f[];
-    __shared__ int tmp[kBfThreads / 32];
+    __shared__ int tmp[kBfThreads / 16];
     __shared__ Unit ring[kBaRing];
     float* q_s = smem_f + T::kStages * T::kStage;
     float* p_s = q_s + T::kQ;                       // [row][kPitchV] scores, then probabilities
     float* m_s = p_s + T::kScores;
     float* l_s = m_s + kBaRows;
     float* f_s = l_s + kBaRows;                     // what a row's output so far is multiplied by
-    int* seg_s = reinterpret_cast<int*>(f_s + kBaRows);
+    Segment* seg = reinterpret_cast<Segment*>(f_s + kBaRows);
+    int* lens = reinterpret_cast<int*>(seg + a.n_segments + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int kvh = blockIdx.y, rep = a.n_heads / a.n_kv_heads, per_part = a.sub_beams + 1;
-    pdl_launch_dependents();
+    const int kvh = blockIdx.y, rep = a.n_heads / a.n_kv_heads;
     pdl_wait();
-    make_plan<kBfThreads>(a, n_segments, seg_s, tmp);
-    const int all = seg_s[n_segments], per = max(1, (all + (int)gridDim.x - 1) / (int)gridDim.x);
-    if (blockIdx.x == 0 && kvh == 0) {
-        for (int s = tid; s <= n_segments; s += kBfThreads) a.plan[1 + s] = seg_s[s];
-        if (tid == 0) a.plan[0] = per;
-    }
-    const int u0 = blockIdx.x * per, u1 = min(all, u0 + per);
+    pdl_launch_dependents();
+    take_plan<kBfThreads>(a, seg, lens, tmp);
+    const int per = stretch_of(seg[a.n_segments].at, gridDim.x);
+    const int u0 = pages_before(a, seg, blockIdx.x * per), u1 = pages_before(a, seg, (blockIdx.x + 1) * per);
     if (u0 >= u1) return;
 
     const size_t page_elements = (size_t)a.n_kv_heads * kPageTokens * D, head_off = (size_t)kvh * kPageTokens * D;
     const uint32_t stage0 = (uint32_t)__cvta_generic_to_shared(smem_f);
     auto know = [&](int u) {
-        if (tid < kBaKnown && u + tid < u1) ring[(u + tid - u0) % kBaRing] = unit_of(a, seg_s, n_segments, u + tid);
+        if (tid < kBaKnown && u + tid < u1) ring[(u + tid - u0) % kBaRing] = unit_of(a, seg, lens, u + tid);
     };
     auto issue = [&](int u) {
         if (u < u1) {
@@ -505,7 +578,7 @@ __global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const _
     float o[T::kRowsEach];
     int segment = -1, part_of = -1, rows = 0, q_row = 0, lo_max = 0, own_row = -1, r0 = 0;
     auto leave = [&]() {
-        const size_t piece = (size_t)kvh * (gridDim.x + n_segments) + blockIdx.x + segment;
+        const size_t piece = (size_t)kvh * (gridDim.x + a.n_segments) + blockIdx.x + segment;
         float* to = a.part_o + piece * kBaRows * D;
         if (row_group < T::kRowGroups) {
 #pragma unroll
@@ -532,7 +605,7 @@ __global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const _
             segment = x.segment;
 #pragma unroll
             for (int j = 0; j < T::kRowsEach; ++j) o[j] = 0.f;
-            const int p = segment / per_part, i = segment % per_part, n = part_rows(a, p);
+            const int p = part_of_segment(a, segment), i = segment - p * (a.sub_beams + 1), n = part_rows(a, p);
             r0 = part_first_row(a, p);
             __syncthreads();        // (the rows' m and l, and the queries, have been read)
             if (p != part_of) {
@@ -549,8 +622,8 @@ __global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const _
             own_row = i == 0 ? -1 : r0 + i - 1;
             for (int r = tid; r < kBaRows; r += kBfThreads) { m_s[r] = -INFINITY; l_s[r] = 0.f; }
             lo_max = 0;
-            if (i == 0) for (int b = 0; b < n; ++b) lo_max = max(lo_max, first_key(a.kv_lens[r0 + b], a.window));
-            else lo_max = first_key(a.kv_lens[own_row], a.window);
+            if (i == 0) for (int b = 0; b < n; ++b) lo_max = max(lo_max, first_key(lens[r0 + b], a.window));
+            else lo_max = first_key(lens[own_row], a.window);
             __syncthreads();
         }
         const float* k_tile = smem_f + ((u - u0) % T::kStages) * T::kStage;
@@ -571,7 +644,7 @@ __global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const _
                 float s = ((s0 + s1) + (s2 + s3)) * scale;
                 if (masked) {
                     const int seq = own_row >= 0 ? own_row : r0 + r / rep, at = x.position + key;
-                    if (key >= x.keys || at < first_key(a.kv_lens[seq], a.window)) s = -INFINITY;
+                    if (key >= x.keys || at < first_key(lens[seq], a.window)) s = -INFINITY;
                 }
                 p_s[r * T::kPitchV + key] = s;
             }
@@ -615,56 +688,63 @@ __global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const _
     leave();
 }
 
-// A warp per (sequence, query head): the pieces that hold the row, first those of the shared pages, then of its own.
+// A warp per (sequence, query head): the pieces that hold the row, first those of the shared pages, then of its own.  A lane reads a piece's maximum
+// and sum; the outputs are asked for eight pieces at a time.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_constant__ BeamAttnArgs a, int n_segments, int n_ctas) {
-    constexpr int E = D / 32;
+__global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_constant__ BeamAttnArgs a, int n_ctas) {
+    constexpr int E = D / 32, kAtOnce = 8;
     // maxima are in units of log 2 where the scores were, in bfloat16
-    auto power = [](float x) { return sizeof(T) == 2 ? exp2f(x) : expf(x); };
+    auto power = [](float x) { return sizeof(T) == 2 ? exp2_fast(x) : expf(x); };
+    const int lane = threadIdx.x & 31, at = blockIdx.x * 4 + (threadIdx.x >> 5), rep = a.n_heads / a.n_kv_heads;
+    const int seq = at / a.n_heads, head = at - seq * a.n_heads, kvh = head / rep, in_group = head - kvh * rep;
+    const int g = seq / a.beams, beam = seq - g * a.beams, sub = a.n_sub == 1 ? 0 : beam / a.sub_beams, i = beam - sub * a.sub_beams;
+    const int shared = (g * a.n_sub + sub) * (a.sub_beams + 1), own = shared + 1 + i;
+    const bool mine = at < a.n_seqs * a.n_heads;
     pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (at >= (long long)a.n_seqs * a.n_heads) return;
-    const int seq = (int)(at / a.n_heads), head = (int)(at % a.n_heads), rep = a.n_heads / a.n_kv_heads, kvh = head / rep;
-    const int g = seq / a.beams, beam = seq % a.beams, p = g * a.n_sub + beam / a.sub_beams, i = beam % a.sub_beams;
-    const int s = p * (a.sub_beams + 1), per = a.plan[0];
-    const size_t base = (size_t)kvh * (n_ctas + n_segments);
+    if (!a.given) pdl_wait();       // (a given plan was complete before the kernel ahead of this one began its work)
+    const Segment* seg = reinterpret_cast<const Segment*>(a.plan);
+    const int line = seg[a.n_segments].at, per = stretch_of(line, n_ctas);
+    int c0 = 0, n0 = 0, c1 = 0, n1 = 0;     // the first CTA with pages of the shared segment and their number; the same of its own
+    if (mine) {
+        const int s0 = seg[shared].pages, s1 = seg[shared + 1].pages, o0 = seg[own].pages, o1 = seg[own + 1].pages;
+        const int sa = seg[shared].at + kSegmentCost, oa = seg[own].at + kSegmentCost;
+        c0 = sa / per;
+        n0 = s0 < s1 ? (sa + s1 - s0 - 1) / per - c0 + 1 : 0;
+        c1 = oa / per;
+        n1 = o0 < o1 ? (oa + o1 - o0 - 1) / per - c1 + 1 : 0;
+    }
+    if (a.given) pdl_wait();
+    if (!mine) return;
+    const int n = n0 + n1;
+    const size_t base = (size_t)kvh * (n_ctas + a.n_segments);
+    auto row_of = [&](int k) {          // of the row in its k-th piece
+        return k < n0 ? (base + c0 + k + shared) * kBaRows + i * rep + in_group : (base + c1 + (k - n0) + own) * kBaRows + in_group;
+    };
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int k0 = 0; k0 < n; k0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (k0 + lane < n) ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * row_of(k0 + lane));
+        const float top = fmaxf(m, warp_max(ml.x)), zero = top == -INFINITY ? 0.f : top, keep = power(m - zero), f = power(ml.x - zero);
+        l = l * keep + warp_sum(ml.y * f);
+        m = top;
 #pragma unroll
-    for (int own = 0; own < 2; ++own) {
-        const int segment = own ? s + 1 + i : s, row = own ? head % rep : i * rep + head % rep;
-        const int first = a.plan[1 + segment], end = a.plan[2 + segment];
-        if (first >= end) continue;
-        const int c0 = first / per, c1 = (end - 1) / per;
-        for (int c = c0; c <= c1; c += 4) {
-            float mc[4], lc[4], oc[4][E];
+        for (int e = 0; e < E; ++e) o[e] *= keep;
+        for (int k1 = 0; k1 < min(32, n - k0); k1 += kAtOnce) {
+            float v[kAtOnce][E];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const size_t piece = (base + min(c + k, c1) + segment) * kBaRows + row;
-                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * piece);
-                mc[k] = c + k <= c1 ? ml.x : -INFINITY;
-                lc[k] = c + k <= c1 ? ml.y : 0.f;
+            for (int k = 0; k < kAtOnce; ++k) {
+                const float* from = a.part_o + row_of(min(k0 + k1 + k, n - 1)) * D + lane;
 #pragma unroll
-                for (int e = 0; e < E; ++e) oc[k][e] = a.part_o[piece * D + e * 32 + lane];
+                for (int e = 0; e < E; ++e) v[k][e] = from[e * 32];
             }
-            float top = m;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top = fmaxf(top, mc[k]);
-            const float zero = top == -INFINITY ? 0.f : top, keep = power(m - zero);
-            l *= keep;
+            for (int k = 0; k < kAtOnce; ++k) {
+                const float w = __shfl_sync(0xffffffffu, f, k1 + k);      // (0 behind the last piece)
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= keep;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float f = power(mc[k] - zero);
-                l += lc[k] * f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] += f > 0.f ? oc[k][e] * f : 0.f;
+                for (int e = 0; e < E; ++e) o[e] += v[k][e] * w;
             }
-            m = top;
         }
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;      // (a sequence without keys: zeros)
@@ -685,13 +765,30 @@ static long long segments_of(int n_groups, int beams, int rep) {
 }
 static long long scratch_floats_of(int n_groups, int beams, int n_heads, int n_kv_heads, int head_dim, int n_parts) {
     const long long segments = segments_of(n_groups, beams, n_heads / n_kv_heads);
-    return (segments + n_parts) * n_kv_heads * kBaRows * (head_dim + 2) + ((segments + 2 + 3) / 4) * 4;
+    return (segments + n_parts) * n_kv_heads * kBaRows * (head_dim + 2) + 4 * (segments + 1);
+}
+static int fill_args(BeamAttnArgs& a, const int* kv_lens, const int* shared_pages, int table_stride, int n_groups, int beams, int n_heads, int n_kv_heads,
+                     int window) {
+    if (beams < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads != 0 || window < 0 || table_stride < 1) return kErrBadArgument;
+    const int rep = n_heads / n_kv_heads;
+    if (rep > 16 || n_kv_heads > 65535) return kErrUnsupportedSize;
+    if (segments_of(n_groups, beams, rep) > kBaMaxSegments) return kErrUnsupportedSize;
+    a = BeamAttnArgs{};
+    a.kv_lens = kv_lens; a.shared_pages = shared_pages;
+    a.table_stride = table_stride; a.n_seqs = n_groups * beams; a.n_groups = n_groups; a.beams = beams;
+    a.sub_beams = beams_of_part(beams, rep);
+    a.n_sub = (beams + a.sub_beams - 1) / a.sub_beams;
+    a.n_parts = n_groups * a.n_sub; a.n_segments = (int)segments_of(n_groups, beams, rep);
+    a.per_magic = (unsigned)(((1ull << 32) + a.sub_beams) / (a.sub_beams + 1));
+    a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.window = window;
+    return 0;
 }
 
+constexpr int kSmShared = 228 * 1024, kCtaShared = 227 * 1024, kCtaReserved = 1024;      // bytes of an SM, the most of a CTA's, what each takes besides
+
 template <typename Kernel>
-static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int, int), int threads, int smem, int (&configured)[64], const BeamAttnArgs& a,
-                        int n_segments, int n_parts, cudaStream_t stream) {
-    smem += (n_segments + 1) * 4;
+static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int), int threads, int smem, int (&configured)[64], const BeamAttnArgs& a, int n_ctas,
+                        cudaStream_t stream) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
     if (configured[device] < smem) {
@@ -699,59 +796,97 @@ static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int, int
         if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
         configured[device] = smem;
     }
-    const int st = launch_pdl(kernel, dim3(n_parts, a.n_kv_heads), dim3(threads), smem, stream, a, n_segments);
+    const int st = launch_pdl(kernel, dim3(n_ctas, a.n_kv_heads), dim3(threads), smem, stream, a);
     if (st != 0) return st;
     const long long rows = (long long)a.n_seqs * a.n_heads;
-    return launch_pdl(join, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, a, n_segments, n_parts);
+    return launch_pdl(join, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, a, n_ctas);
+}
+
+// bytes of dynamic shared memory with that many stages
+template <int D>
+static int beam_smem(const BeamAttnArgs& a, int stages) {
+    return stages * BeamTile<D>::kStage + a.sub_beams * (a.n_heads / a.n_kv_heads) * BeamTile<D>::kPitchK + plan_ints(a) * 4;
 }
 
 template <int D>
-static int launch_beams_of(int dtype, const BeamAttnArgs& a, int n_segments, int n_parts, cudaStream_t stream) {
-    static int configured[64] = {}, configured_f32[64] = {};
-    if (dtype == kBF16)
-        return launch_beams(attention_beams_kernel<D>, attention_beams_join_kernel<__nv_bfloat16, D>, kBaThreads, BeamTile<D>::kBytes, configured, a,
-                            n_segments, n_parts, stream);
-    return launch_beams(attention_beams_f32_kernel<D>, attention_beams_join_kernel<float, D>, kBfThreads, BeamTileF32<D>::kBytes, configured_f32, a,
-                        n_segments, n_parts, stream);
+static int launch_beams_of(int dtype, const BeamAttnArgs& a, int n_ctas, cudaStream_t stream) {
+    static int configured[3][64] = {};
+    const auto join = dtype == kBF16 ? attention_beams_join_kernel<__nv_bfloat16, D> : attention_beams_join_kernel<float, D>;
+    if (dtype == kF32) {
+        const int smem = BeamTileF32<D>::kBytes + plan_ints(a) * 4;
+        if (smem + 2048 > kCtaShared) return kErrUnsupportedSize;
+        return launch_beams(attention_beams_f32_kernel<D>, join, kBfThreads, smem, configured[0], a, n_ctas, stream);
+    }
+    // As many stages as leave room for three CTAs an SM with heads of up to 64, two with wider ones.
+    constexpr int kMore = D <= 64 ? 4 : 3, kResident = D <= 64 ? 3 : 2, kStatic = 16 + kBaRing * (int)sizeof(Unit);
+    const int smem = beam_smem<D>(a, kMore);
+    if (smem + kStatic + kCtaReserved <= kSmShared / kResident)
+        return launch_beams(attention_beams_kernel<D, kMore>, join, kBaThreads, smem, configured[1], a, n_ctas, stream);
+    return launch_beams(attention_beams_kernel<D, 2>, join, kBaThreads, beam_smem<D>(a, 2), configured[2], a, n_ctas, stream);
 }
 
 }  // namespace b200
 
 extern "C" long long b200_attention_beams_scratch_floats(int n_groups, int beams, int n_heads, int n_kv_heads, int head_dim, int n_parts) {
-    if (n_groups < 1 || beams < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || n_heads / n_kv_heads > b200::kBaRows) return 0;
+    if (n_groups < 1 || beams < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || n_heads / n_kv_heads > 16) return 0;
     return b200::scratch_floats_of(n_groups, beams, n_heads, n_kv_heads, head_dim, n_parts);
 }
 
+// Ints of a plan (see below) for so many sequences in groups.
+extern "C" int b200_attention_beams_plan_ints(int n_groups, int beams, int n_heads, int n_kv_heads) {
+    if (n_groups < 1 || beams < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || n_heads / n_kv_heads > 16) return 0;
+    return (int)(4 * (b200::segments_of(n_groups, beams, n_heads / n_kv_heads) + 1));
+}
+
+// The plan alone, for the layers of a step that share lengths, shared pages, heads and window.
+extern "C" int b200_attention_beams_plan(int* plan, const int* kv_lens, const int* shared_pages, int table_stride, int n_groups, int beams, int n_heads,
+                                         int n_kv_heads, int window, cudaStream_t stream) {
+    using namespace b200;
+    if (n_groups <= 0) return 0;
+    BeamAttnArgs a;
+    const int st = fill_args(a, kv_lens, shared_pages, table_stride, n_groups, beams, n_heads, n_kv_heads, window);
+    if (st != 0) return st;
+    if (((uintptr_t)plan & 15) != 0) return kErrUnsupportedSize;
+    a.plan = plan;
+    static bool configured[64] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
+    const int smem = plan_ints(a) * 4;
+    if (smem > 48 * 1024 && !configured[device]) {
+        const cudaError_t e = cudaFuncSetAttribute(attention_beams_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCtaShared - 1024);
+        if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
+        configured[device] = true;
+    }
+    return launch_pdl(attention_beams_plan_kernel, dim3(1), dim3(256), smem, stream, a);
+}
+
 // Sequences are n_groups groups of `beams`; kv_lens[n_seqs], page_table [n_seqs][table_stride], shared_pages[n_groups].  n_parts: CTAs of
-// a kv head.  Keys and values of the step are in the cache already.
+// a kv head.  plan: null, or what b200_attention_beams_plan made of the same numbers.  Keys and values of the step are in the cache already.
 extern "C" int b200_attention_beams(const void* q, long long q_row_stride, void* out, const int* kv_lens, const int* page_table, int table_stride,
                                     const int* shared_pages, const void* k_pool, const void* v_pool, float* scratch, long long scratch_floats,
                                     int n_groups, int beams, int n_heads, int n_kv_heads, int head_dim, int window, int n_parts,
-                                    int dtype, cudaStream_t stream) {
+                                    int dtype, const int* plan, cudaStream_t stream) {
     using namespace b200;
     if (n_groups <= 0) return 0;
-    if ((dtype != kF32 && dtype != kBF16) || beams < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || window < 0 || n_parts < 1 || table_stride < 1) return kErrBadArgument;
-    const int rep = n_heads / n_kv_heads;
-    if (rep > 16 || head_dim % 32 != 0 || head_dim < 32 || head_dim > 128 || n_kv_heads > 65535 || n_parts > 65535) return kErrUnsupportedSize;
-    const long long segments = segments_of(n_groups, beams, rep);
-    if (segments > kBaMaxSegments) return kErrUnsupportedSize;
-    if (q_row_stride % (dtype == kBF16 ? 8 : 4) != 0 || (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)scratch) & 15) != 0) return kErrUnsupportedSize;
-    if (scratch_floats < scratch_floats_of(n_groups, beams, n_heads, n_kv_heads, head_dim, n_parts)) return 10003;
     BeamAttnArgs a;
-    a.q = q; a.out = out; a.kv_lens = kv_lens; a.page_table = page_table; a.shared_pages = shared_pages; a.k_pool = k_pool; a.v_pool = v_pool;
-    const long long pieces = (segments + n_parts) * n_kv_heads;
+    const int st = fill_args(a, kv_lens, shared_pages, table_stride, n_groups, beams, n_heads, n_kv_heads, window);
+    if (st != 0) return st;
+    if ((dtype != kF32 && dtype != kBF16) || n_parts < 1) return kErrBadArgument;
+    if (head_dim % 32 != 0 || head_dim < 32 || head_dim > 128 || n_parts > 65535 || (long long)a.n_seqs * n_heads > (1 << 28)) return kErrUnsupportedSize;
+    if (q_row_stride % (dtype == kBF16 ? 8 : 4) != 0 || (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)scratch | (uintptr_t)plan) & 15) != 0)
+        return kErrUnsupportedSize;
+    if (scratch_floats < scratch_floats_of(n_groups, beams, n_heads, n_kv_heads, head_dim, n_parts)) return 10003;
+    a.q = q; a.out = out; a.page_table = page_table; a.k_pool = k_pool; a.v_pool = v_pool;
+    a.q_row_stride = q_row_stride;
+    const long long pieces = (long long)(a.n_segments + n_parts) * n_kv_heads;
     a.part_o = scratch;
     a.part_ml = scratch + pieces * kBaRows * head_dim;
-    a.plan = (int*)(a.part_ml + pieces * kBaRows * 2);
-    a.q_row_stride = q_row_stride;
-    a.table_stride = table_stride; a.n_seqs = n_groups * beams; a.n_groups = n_groups; a.beams = beams;
-    a.sub_beams = beams_of_part(beams, rep);
-    a.n_sub = (beams + a.sub_beams - 1) / a.sub_beams;
-    a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.window = window;
+    a.given = plan != nullptr;
+    a.plan = plan ? const_cast<int*>(plan) : (int*)(a.part_ml + pieces * kBaRows * 2);
     switch (head_dim) {
-        case 32: return launch_beams_of<32>(dtype, a, (int)segments, n_parts, stream);
-        case 64: return launch_beams_of<64>(dtype, a, (int)segments, n_parts, stream);
-        case 96: return launch_beams_of<96>(dtype, a, (int)segments, n_parts, stream);
-        default: return launch_beams_of<128>(dtype, a, (int)segments, n_parts, stream);
+        case 32: return launch_beams_of<32>(dtype, a, n_parts, stream);
+        case 64: return launch_beams_of<64>(dtype, a, n_parts, stream);
+        case 96: return launch_beams_of<96>(dtype, a, n_parts, stream);
+        default: return launch_beams_of<128>(dtype, a, n_parts, stream);
     }
 }

@@ -176,7 +176,8 @@ _SIGNATURES = {
                                        c_int, c_void_p]),
     "b200_attention_beams": ("attention_beams", [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                                  c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_int, c_int,
-                                                 c_int, c_int]),
+                                                 c_int, c_int, c_void_p]),
+    "b200_attention_beams_plan": ("attention_beams", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int]),
     "b200_sample_rows": ("sampling", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_float, c_void_p]),
 }
 
@@ -1261,13 +1262,34 @@ def attention_beams_parts(n_groups: int, beams: int, n_heads: int, n_kv_heads: i
     return max(1, min(per_sm * sm_count(torch.device(device)) // n_kv_heads, pages))
 
 
+def attention_beams_plan(kv_lens: torch.Tensor, shared_pages: torch.Tensor, table_width: int, n_heads: int, n_kv_heads: int, window: int,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """How the pages of a step's groups are shared out (int32), for several calls of ``attention_decode_beams`` in that step."""
+    _here(kv_lens, shared_pages, out)
+    n_seqs, n_groups = kv_lens.numel(), shared_pages.numel()
+    assert kv_lens.dtype == shared_pages.dtype == torch.int32 and kv_lens.is_contiguous() and shared_pages.is_contiguous()
+    if n_groups == 0 or n_seqs % n_groups:
+        raise KernelError(f"{n_seqs} sequences do not make {n_groups} equal groups")
+    size = library("attention_beams").b200_attention_beams_plan_ints
+    size.argtypes, size.restype = [c_int] * 4, c_int
+    need = int(size(n_groups, n_seqs // n_groups, n_heads, n_kv_heads))
+    if out is None:
+        out = torch.empty(need, dtype=torch.int32, device=kv_lens.device)
+    assert out.dtype == torch.int32 and out.is_contiguous() and out.numel() >= need
+    _check(_fn("b200_attention_beams_plan")(out.data_ptr(), kv_lens.data_ptr(), shared_pages.data_ptr(), int(table_width), n_groups,
+                                            n_seqs // n_groups, n_heads, n_kv_heads, int(window), _stream()), "attention_beams_plan")
+    return out
+
+
 def attention_decode_beams(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor,
                            shared_pages: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, n_heads: int, n_kv_heads: int,
-                           head_dim: int, window: int, n_parts: int, scratch: torch.Tensor | None = None) -> None:
+                           head_dim: int, window: int, n_parts: int, scratch: torch.Tensor | None = None, *,
+                           plan: torch.Tensor | None = None) -> None:
     """``attention_decode`` for sequences in groups of equal size that share their first pages (the beams of a request): group g is
     sequences g B .. (g + 1) B - 1, and the first shared_pages[g] entries of their rows of the page table are the same (int32 [groups]; pages
-    that are not full for all of the group's sequences count as each one's own).  ``n_parts``: see ``attention_beams_parts``."""
-    _here(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, scratch)
+    that are not full for all of the group's sequences count as each one's own).  ``n_parts``: see ``attention_beams_parts``.  ``plan``: what
+    ``attention_beams_plan`` made of the same lengths, shared pages, heads, window and width of the page table."""
+    _here(plan, q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, scratch)
     n_seqs, n_groups = out.shape[0], shared_pages.numel()
     if not attention_beams_supported(q.dtype, n_heads, n_kv_heads, head_dim):
         raise KernelError(f"attention_decode_beams: {n_heads} heads on {n_kv_heads} of {head_dim} in {q.dtype}")
@@ -1292,7 +1314,7 @@ def attention_decode_beams(q: torch.Tensor, q_row_stride: int, out: torch.Tensor
     _check(_fn("b200_attention_beams")(
         q.data_ptr(), q_row_stride, out.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), page_table.shape[1], shared_pages.data_ptr(),
         k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), n_groups, B, n_heads, n_kv_heads, head_dim, int(window),
-        n_parts, dtype_code(q.dtype), _stream()), "attention_decode_beams")
+        n_parts, dtype_code(q.dtype), plan.data_ptr() if plan is not None else None, _stream()), "attention_decode_beams")
 
 
 # --------------------------------------------------------------------------- several residual streams
