@@ -15,6 +15,10 @@
 // scratch at the segment's end or its own; a second kernel joins what the CTAs left of a row, in a fixed order.  CTA c's piece of
 // segment s is number c + s (along the pages either grows, so no two pieces have one number).
 //
+// Fused variant (b200_attention_beams_rope): the step's own rotation and cache write are done here, as in the decode kernel for separate
+// sequences: the queries are turned on their way into shared memory, and the CTA that meets a sequence's last page turns the new key, puts it and the new
+// value into the page as it lies in shared memory and into the cache.  The page that holds the new position is always a sequence's own.
+//
 // Groups of more than 64 rows to a kv head are cut into equal groups of whole beams, each of which reads the shared pages.
 #include "common.cuh"
 
@@ -37,6 +41,10 @@ struct BeamAttnArgs {
     float* part_ml;                     // [kv_head][piece][row][2]
     int* plan;                          // the segments, as many ints as plan_ints
     int given;                          // whether they are there already
+    const float* inv_freq;              // of the fused variant, [head_dim / 2], else null
+    int pairing;                        // 0: (2j, 2j+1); 1: (j, j + head_dim/2)
+    int write_cache;                    // whether the step's keys and values go into the cache here
+    int fresh;                          // 1: the last position's key and value are not in the cache yet
     unsigned per_magic;                 // 2^32 / (sub_beams + 1), rounded up
     long long q_row_stride;
     int table_stride, n_seqs, n_groups, beams, sub_beams, n_sub, n_parts, n_segments, n_heads, n_kv_heads, window;
@@ -51,7 +59,7 @@ __device__ __forceinline__ int part_rows(const BeamAttnArgs& a, int p) { return 
 
 __device__ __forceinline__ int part_of_segment(const BeamAttnArgs& a, int s) { return (int)__umulhi((unsigned)s, a.per_magic); }   // (s below 2^16)
 
-constexpr int kSegmentCost = 1;
+constexpr int kSegmentCost = 2;
 struct Segment {
     int pages;          // pages before it
     int at;             // where it begins on the line
@@ -77,7 +85,7 @@ __device__ __forceinline__ void make_plan(const BeamAttnArgs& a, Segment* seg, i
         const int r0 = part_first_row(a, p), n = part_rows(a, p);
         int shortest = lens[r0];
         for (int i = 1; i < n; ++i) shortest = min(shortest, lens[r0 + i]);
-        const int hi = min(range[2 * p + 1], shortest / kPageTokens);
+        const int hi = min(range[2 * p + 1], max(shortest - a.fresh, 0) / kPageTokens);
         range[2 * p] = min(first_key(shortest, a.window) / kPageTokens, hi);
         range[2 * p + 1] = hi;
     }
@@ -382,7 +390,8 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
     unsigned char* q_s = smem + STAGES * T::kStage;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int kvh = blockIdx.y, rep = a.n_heads / a.n_kv_heads;
-    Segment* seg = reinterpret_cast<Segment*>(q_s + a.sub_beams * rep * T::kPitchK);
+    float* turn_s = reinterpret_cast<float*>(q_s + a.sub_beams * rep * T::kPitchK);     // fused: [sequence of the part][cosines, sines of its D / 2 angles]
+    Segment* seg = reinterpret_cast<Segment*>(turn_s + (a.inv_freq ? a.sub_beams * D : 0));
     int* lens = reinterpret_cast<int*>(seg + a.n_segments + 1);
     pdl_wait();
     // (only now: the kernel that joins the pieces may read a given plan as soon as it starts)
@@ -423,8 +432,42 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
         }
         cp_async_commit();
     };
+    auto turned = [&](const float* turn, float x0, float x1, int j, float& y0, float& y1) {
+        const float cs = turn[j], sn = turn[D / 2 + j];
+        y0 = __fmaf_rn(x0, cs, -__fmul_rn(x1, sn));     // (the second product is rounded: queries and keys alike, wherever they are turned)
+        y1 = __fmaf_rn(x0, sn, __fmul_rn(x1, cs));
+    };
     auto ask_queries = [&](int p) {     // of all rows of part p
         const int r0 = part_first_row(a, p);
+        if (a.inv_freq) {
+            const int n = part_rows(a, p);
+            for (int c = tid; c < n * (D / 2); c += kBaThreads) {
+                const int b = c / (D / 2), j = c % (D / 2);
+                sincosf((float)(lens[r0 + b] - 1) * a.inv_freq[j], &turn_s[b * D + D / 2 + j], &turn_s[b * D + j]);
+            }
+            __syncthreads();
+            // two pieces of a row at a time: neighbours, or a half row apart
+            for (int c = tid; c < n * rep * (CK / 2); c += kBaThreads) {
+                const int row = c / (CK / 2), at = c % (CK / 2), first = a.pairing == 0 ? 2 * at : at, second = a.pairing == 0 ? 2 * at + 1 : at + CK / 2;
+                const __nv_bfloat16* from = (const __nv_bfloat16*)a.q + (size_t)(r0 + row / rep) * a.q_row_stride + (size_t)(kvh * rep + row % rep) * D;
+                const uint4 x = *reinterpret_cast<const uint4*>(from + first * 8), y = *reinterpret_cast<const uint4*>(from + second * 8);
+                const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                float v[16];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { v[2 * k] = __uint_as_float(w[k] << 16); v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
+                const float* turn = turn_s + row / rep * D;
+                if (a.pairing == 0) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) turned(turn, v[2 * k], v[2 * k + 1], at * 8 + k, v[2 * k], v[2 * k + 1]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) turned(turn, v[k], v[8 + k], at * 8 + k, v[k], v[8 + k]);
+                }
+                *reinterpret_cast<uint4*>(q_s + T::k_piece(row, first)) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+                *reinterpret_cast<uint4*>(q_s + T::k_piece(row, second)) = make_uint4(pack2(v[8], v[9]), pack2(v[10], v[11]), pack2(v[12], v[13]), pack2(v[14], v[15]));
+            }
+            return;
+        }
         for (int c = tid; c < part_rows(a, p) * rep * CK; c += kBaThreads) {
             const int row = c / CK, at = c % CK;
             cp_async16(q_base + T::k_piece(row, at), (const __nv_bfloat16*)a.q + (size_t)(r0 + row / rep) * a.q_row_stride
@@ -434,9 +477,10 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
     know(u0);
     __syncthreads();
     int part_of = part_of_segment(a, ring[0].segment);
-    ask_queries(part_of);               // (they arrive with the first page)
+    if (!a.inv_freq) ask_queries(part_of);               // (they arrive with the first page)
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) issue(u0 + i);
+    if (a.inv_freq) ask_queries(part_of);                // (made while the first pages are on their way)
 
     const float scale_log2 = 1.4426950408889634f / sqrtf((float)D);
     RowState<D> st;
@@ -490,6 +534,30 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
             __syncthreads();
         }
         issue(ahead);
+        if (a.write_cache && row_end - x.position <= kPageTokens) {      // a sequence's last page: its new key and value
+            const Segment own = seg[segment];
+            const int slot = (u - u0) % STAGES, new_at = x.keys - 1, beam = own.row - part_first_row(a, part_of);
+            const __nv_bfloat16* k_raw = (const __nv_bfloat16*)a.q + (size_t)own.row * a.q_row_stride + (size_t)(a.n_heads + kvh) * D;
+            const __nv_bfloat16* v_raw = k_raw + (size_t)a.n_kv_heads * D;
+            __nv_bfloat16* k = (__nv_bfloat16*)a.k_pool + (size_t)x.page * page_elements + head_off + (size_t)new_at * D;
+            __nv_bfloat16* v = (__nv_bfloat16*)a.v_pool + (size_t)x.page * page_elements + head_off + new_at;
+            unsigned char* ks = smem + slot * T::kStage;
+            unsigned char* vs = ks + kPageTokens * T::kPitchK;
+            for (int j = tid; j < D / 2; j += kBaThreads) {
+                const int d[2] = {a.pairing == 0 ? 2 * j : j, a.pairing == 0 ? 2 * j + 1 : j + D / 2};
+                float y[2];
+                turned(turn_s + beam * D, __bfloat162float(k_raw[d[0]]), __bfloat162float(k_raw[d[1]]), j, y[0], y[1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const __nv_bfloat16 key = __float2bfloat16_rn(y[e]), value = v_raw[d[e]];
+                    k[d[e]] = key;
+                    v[(size_t)d[e] * kPageTokens] = value;
+                    *reinterpret_cast<__nv_bfloat16*>(ks + T::k_piece(new_at, d[e] / 8) + (d[e] % 8) * 2) = key;
+                    *reinterpret_cast<__nv_bfloat16*>(vs + T::v_piece(d[e], new_at / 8) + (new_at % 8) * 2) = value;
+                }
+            }
+            __syncthreads();
+        }
         if (tile * 16 < rows) {
             const uint32_t ks = stage0 + (uint32_t)(((u - u0) % STAGES) * T::kStage), vs = ks + kPageTokens * T::kPitchK;
             const bool masked = x.keys < kPageTokens || x.position < lo_max;
@@ -805,7 +873,7 @@ static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int), in
 // bytes of dynamic shared memory with that many stages
 template <int D>
 static int beam_smem(const BeamAttnArgs& a, int stages) {
-    return stages * BeamTile<D>::kStage + a.sub_beams * (a.n_heads / a.n_kv_heads) * BeamTile<D>::kPitchK + plan_ints(a) * 4;
+    return stages * BeamTile<D>::kStage + a.sub_beams * ((a.n_heads / a.n_kv_heads) * BeamTile<D>::kPitchK + (a.inv_freq ? D * 4 : 0)) + plan_ints(a) * 4;
 }
 
 template <int D>
@@ -838,9 +906,10 @@ extern "C" int b200_attention_beams_plan_ints(int n_groups, int beams, int n_hea
     return (int)(4 * (b200::segments_of(n_groups, beams, n_heads / n_kv_heads) + 1));
 }
 
-// The plan alone, for the layers of a step that share lengths, shared pages, heads and window.
+// The plan alone, for the layers of a step that share lengths, shared pages, heads and window.  fresh: 1 for the fused variant that writes the
+// cache (the page that holds the last position is then no shared one, whatever shared_pages says).
 extern "C" int b200_attention_beams_plan(int* plan, const int* kv_lens, const int* shared_pages, int table_stride, int n_groups, int beams, int n_heads,
-                                         int n_kv_heads, int window, cudaStream_t stream) {
+                                         int n_kv_heads, int window, int fresh, cudaStream_t stream) {
     using namespace b200;
     if (n_groups <= 0) return 0;
     BeamAttnArgs a;
@@ -848,6 +917,7 @@ extern "C" int b200_attention_beams_plan(int* plan, const int* kv_lens, const in
     if (st != 0) return st;
     if (((uintptr_t)plan & 15) != 0) return kErrUnsupportedSize;
     a.plan = plan;
+    a.fresh = fresh != 0;
     static bool configured[64] = {};
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
@@ -860,24 +930,24 @@ extern "C" int b200_attention_beams_plan(int* plan, const int* kv_lens, const in
     return launch_pdl(attention_beams_plan_kernel, dim3(1), dim3(256), smem, stream, a);
 }
 
-// Sequences are n_groups groups of `beams`; kv_lens[n_seqs], page_table [n_seqs][table_stride], shared_pages[n_groups].  n_parts: CTAs of
-// a kv head.  plan: null, or what b200_attention_beams_plan made of the same numbers.  Keys and values of the step are in the cache already.
-extern "C" int b200_attention_beams(const void* q, long long q_row_stride, void* out, const int* kv_lens, const int* page_table, int table_stride,
-                                    const int* shared_pages, const void* k_pool, const void* v_pool, float* scratch, long long scratch_floats,
-                                    int n_groups, int beams, int n_heads, int n_kv_heads, int head_dim, int window, int n_parts,
-                                    int dtype, const int* plan, cudaStream_t stream) {
-    using namespace b200;
+namespace b200 {
+
+static int attention_beams(const void* q, long long q_row_stride, void* out, const int* kv_lens, const int* page_table, int table_stride,
+                           const int* shared_pages, const void* k_pool, const void* v_pool, float* scratch, long long scratch_floats, int n_groups, int beams,
+                           int n_heads, int n_kv_heads, int head_dim, int window, int n_parts, int dtype, const int* plan, const float* inv_freq, int pairing,
+                           int write_cache, cudaStream_t stream) {
     if (n_groups <= 0) return 0;
     BeamAttnArgs a;
     const int st = fill_args(a, kv_lens, shared_pages, table_stride, n_groups, beams, n_heads, n_kv_heads, window);
     if (st != 0) return st;
-    if ((dtype != kF32 && dtype != kBF16) || n_parts < 1) return kErrBadArgument;
+    if ((dtype != kF32 && dtype != kBF16) || n_parts < 1 || pairing < 0 || pairing > 1) return kErrBadArgument;
     if (head_dim % 32 != 0 || head_dim < 32 || head_dim > 128 || n_parts > 65535 || (long long)a.n_seqs * n_heads > (1 << 28)) return kErrUnsupportedSize;
     if (q_row_stride % (dtype == kBF16 ? 8 : 4) != 0 || (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)scratch | (uintptr_t)plan) & 15) != 0)
         return kErrUnsupportedSize;
     if (scratch_floats < scratch_floats_of(n_groups, beams, n_heads, n_kv_heads, head_dim, n_parts)) return 10003;
     a.q = q; a.out = out; a.page_table = page_table; a.k_pool = k_pool; a.v_pool = v_pool;
     a.q_row_stride = q_row_stride;
+    a.inv_freq = inv_freq; a.pairing = pairing; a.write_cache = inv_freq && write_cache; a.fresh = a.write_cache;
     const long long pieces = (long long)(a.n_segments + n_parts) * n_kv_heads;
     a.part_o = scratch;
     a.part_ml = scratch + pieces * kBaRows * head_dim;
@@ -889,4 +959,27 @@ extern "C" int b200_attention_beams(const void* q, long long q_row_stride, void*
         case 96: return launch_beams_of<96>(dtype, a, n_parts, stream);
         default: return launch_beams_of<128>(dtype, a, n_parts, stream);
     }
+}
+
+}  // namespace b200
+
+// Sequences are n_groups groups of `beams`; kv_lens[n_seqs], page_table [n_seqs][table_stride], shared_pages[n_groups].  n_parts: CTAs of
+// a kv head.  plan: null, or what b200_attention_beams_plan made of the same numbers.  Keys and values of the step are in the cache already.
+extern "C" int b200_attention_beams(const void* q, long long q_row_stride, void* out, const int* kv_lens, const int* page_table, int table_stride,
+                                    const int* shared_pages, const void* k_pool, const void* v_pool, float* scratch, long long scratch_floats,
+                                    int n_groups, int beams, int n_heads, int n_kv_heads, int head_dim, int window, int n_parts,
+                                    int dtype, const int* plan, cudaStream_t stream) {
+    return b200::attention_beams(q, q_row_stride, out, kv_lens, page_table, table_stride, shared_pages, k_pool, v_pool, scratch, scratch_floats, n_groups,
+                                 beams, n_heads, n_kv_heads, head_dim, window, n_parts, dtype, plan, nullptr, 0, 0, stream);
+}
+
+// The fused variant, bfloat16: `qkv` holds the step's raw projections [n_seqs, (n_heads + 2 n_kv_heads) head_dim]; queries are turned here, and with
+// write_cache the new key (turned) and value are stored at position kv_len - 1.  Rotary dimension = head_dim.
+extern "C" int b200_attention_beams_rope(const void* qkv, long long q_row_stride, void* out, const int* kv_lens, const int* page_table, int table_stride,
+                                         const int* shared_pages, void* k_pool, void* v_pool, float* scratch, long long scratch_floats, int n_groups,
+                                         int beams, int n_heads, int n_kv_heads, int head_dim, int window, int n_parts, const int* plan,
+                                         const float* inv_freq, int pairing, int write_cache, cudaStream_t stream) {
+    if (inv_freq == nullptr) return b200::kErrBadArgument;
+    return b200::attention_beams(qkv, q_row_stride, out, kv_lens, page_table, table_stride, shared_pages, k_pool, v_pool, scratch, scratch_floats, n_groups,
+                                 beams, n_heads, n_kv_heads, head_dim, window, n_parts, b200::kBF16, plan, inv_freq, pairing, write_cache, stream);
 }

@@ -58,7 +58,11 @@ def try_decode_attention_with_rope(qkv, out, ctx, page_table, cache, mixer, writ
                                                                    mixer.head_dim, pos.rotary_dim, pos.pairing)):
         return False
     if beams_share_attention(ctx, mixer, qkv.dtype):
-        return False
+        shared, parts, plan = _beam_launch(ctx, page_table, cache, mixer, qkv.dtype, bool(writes_cache))
+        ops.attention_decode_beams_rope(qkv, out, ctx.kv_lens, page_table, shared, cache.k, cache.v, pos.inverse_frequencies(qkv.device),
+                                        mixer.n_heads, mixer.n_kv_heads, mixer.head_dim, pos.pairing, mixer.window or 0, parts,
+                                        write_cache=writes_cache, plan=plan)
+        return True
     splits, early = mixer.plan_decode(ctx, cache)
     ops.attention_decode_rope(qkv, out, ctx.kv_lens, page_table, cache.k, cache.v, pos.inverse_frequencies(qkv.device),
                               mixer.n_heads, mixer.n_kv_heads, mixer.head_dim, pos.pairing, mixer.window or 0, splits,
@@ -73,13 +77,26 @@ def beams_share_attention(ctx, mixer, dtype) -> bool:
             and ops.attention_beams_supported(dtype, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim))
 
 
+def _beam_launch(ctx, page_table, cache, mixer, dtype, writes_cache: bool):
+    """What a call of the attention of groups needs beside its operands: the shared pages, how many CTAs, and the plan, which is made
+    once for all layers of a kind."""
+    shared = ctx.shared_pages[cache.group]
+    parts = ops.attention_beams_parts(ctx.n_seqs // ctx.beams, ctx.beams, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim,
+                                      ctx.capacity(cache.group), dtype, page_table.device)
+    key = ("beam attention", cache.group, mixer.n_heads, mixer.n_kv_heads, mixer.window, writes_cache)
+    plan = ctx.extras.get(key)
+    if plan is None:
+        plan = ctx.extras[key] = ops.attention_beams_plan(ctx.kv_lens, shared, page_table.shape[1], mixer.n_heads, mixer.n_kv_heads,
+                                                          mixer.window or 0, writes_cache=writes_cache)
+    return shared, parts, plan
+
+
 def try_beam_attention(qkv, out, ctx, page_table, cache, mixer, gate=None) -> bool:
     if gate is not None or not beams_share_attention(ctx, mixer, qkv.dtype) or qkv.shape[1] % 8 or qkv.data_ptr() & 15:
         return False
-    parts = ops.attention_beams_parts(ctx.n_seqs // ctx.beams, ctx.beams, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim,
-                                      ctx.capacity(cache.group), qkv.dtype, qkv.device)
-    ops.attention_decode_beams(qkv, qkv.shape[1], out, ctx.kv_lens, page_table, ctx.shared_pages[cache.group], cache.k, cache.v, mixer.n_heads,
-                               mixer.n_kv_heads, mixer.head_dim, mixer.window or 0, parts)
+    shared, parts, plan = _beam_launch(ctx, page_table, cache, mixer, qkv.dtype, False)
+    ops.attention_decode_beams(qkv, qkv.shape[1], out, ctx.kv_lens, page_table, shared, cache.k, cache.v, mixer.n_heads,
+                               mixer.n_kv_heads, mixer.head_dim, mixer.window or 0, parts, plan=plan)
     return True
 
 

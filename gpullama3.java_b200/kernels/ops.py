@@ -177,7 +177,10 @@ _SIGNATURES = {
     "b200_attention_beams": ("attention_beams", [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                                  c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_int, c_int,
                                                  c_int, c_int, c_void_p]),
-    "b200_attention_beams_plan": ("attention_beams", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "b200_attention_beams_rope": ("attention_beams", [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                                      c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_int, c_int,
+                                                      c_int, c_void_p, c_void_p, c_int, c_int]),
+    "b200_attention_beams_plan": ("attention_beams", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "b200_sample_rows": ("sampling", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_float, c_void_p]),
 }
 
@@ -1132,10 +1135,17 @@ BEAM_MAX_KEEP = 256   # beam_select.cu
 
 def _here(*tensors: torch.Tensor) -> None:
     """The tensors lie on the current device, on whose current stream a launch goes."""
-    _dev(*tensors)
+    current = None
     for t in tensors:
-        if t is not None and t.device.index != torch.cuda.current_device():
-            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        if t is None:
+            continue
+        at = t.get_device()         # (-1: no CUDA tensor)
+        if at != current:
+            if at < 0:
+                raise KernelError("kernels take CUDA tensors only; there is no CPU path")
+            if current is not None or at != torch.cuda.current_device():
+                raise KernelError(f"a tensor lies on cuda:{at}, the current device is cuda:{torch.cuda.current_device()}")
+            current = at
 
 
 def beam_select_takes(beams: int, keep: int) -> bool:
@@ -1262,23 +1272,65 @@ def attention_beams_parts(n_groups: int, beams: int, n_heads: int, n_kv_heads: i
     return max(1, min(per_sm * sm_count(torch.device(device)) // n_kv_heads, pages))
 
 
+def _beams_numbers(n_groups: int, beams: int, n_heads: int, n_kv_heads: int, head_dim: int, n_parts: int) -> tuple[int, int]:
+    """Floats of scratch and ints of a plan for such a call."""
+    key = (n_groups, beams, n_heads, n_kv_heads, head_dim, n_parts)
+    found = _beams_sizes.get(key)
+    if found is None:
+        lib = library("attention_beams")
+        floats, ints = lib.b200_attention_beams_scratch_floats, lib.b200_attention_beams_plan_ints
+        floats.argtypes, floats.restype = [c_int] * 6, ctypes.c_longlong
+        ints.argtypes, ints.restype = [c_int] * 4, c_int
+        if len(_beams_sizes) > 1000:
+            _beams_sizes.clear()
+        found = _beams_sizes[key] = (int(floats(*key)), int(ints(*key[:4])))
+    return found
+
+
+_beams_sizes: dict = {}
+
+
 def attention_beams_plan(kv_lens: torch.Tensor, shared_pages: torch.Tensor, table_width: int, n_heads: int, n_kv_heads: int, window: int,
-                         out: torch.Tensor | None = None) -> torch.Tensor:
-    """How the pages of a step's groups are shared out (int32), for several calls of ``attention_decode_beams`` in that step."""
+                         out: torch.Tensor | None = None, *, writes_cache: bool = False) -> torch.Tensor:
+    """How the pages of a step's groups are shared out (int32), for several calls of ``attention_decode_beams`` in that step, or with
+    ``writes_cache`` of ``attention_decode_beams_rope``."""
     _here(kv_lens, shared_pages, out)
     n_seqs, n_groups = kv_lens.numel(), shared_pages.numel()
     assert kv_lens.dtype == shared_pages.dtype == torch.int32 and kv_lens.is_contiguous() and shared_pages.is_contiguous()
     if n_groups == 0 or n_seqs % n_groups:
         raise KernelError(f"{n_seqs} sequences do not make {n_groups} equal groups")
-    size = library("attention_beams").b200_attention_beams_plan_ints
-    size.argtypes, size.restype = [c_int] * 4, c_int
-    need = int(size(n_groups, n_seqs // n_groups, n_heads, n_kv_heads))
+    need = _beams_numbers(n_groups, n_seqs // n_groups, n_heads, n_kv_heads, 64, 1)[1]
     if out is None:
         out = torch.empty(need, dtype=torch.int32, device=kv_lens.device)
     assert out.dtype == torch.int32 and out.is_contiguous() and out.numel() >= need
     _check(_fn("b200_attention_beams_plan")(out.data_ptr(), kv_lens.data_ptr(), shared_pages.data_ptr(), int(table_width), n_groups,
-                                            n_seqs // n_groups, n_heads, n_kv_heads, int(window), _stream()), "attention_beams_plan")
+                                            n_seqs // n_groups, n_heads, n_kv_heads, int(window), 1 if writes_cache else 0, _stream()),
+           "attention_beams_plan")
     return out
+
+
+def _beams_checked(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan):
+    """The checks that both forms share; the number of groups and of sequences in one, and the scratch."""
+    _here(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, scratch, plan)
+    n_seqs, n_groups = out.shape[0], shared_pages.numel()
+    if not attention_beams_supported(q.dtype, n_heads, n_kv_heads, head_dim):
+        raise KernelError(f"attention_decode_beams: {n_heads} heads on {n_kv_heads} of {head_dim} in {q.dtype}")
+    if n_groups == 0 or n_seqs % n_groups:
+        raise KernelError(f"{n_seqs} sequences do not make {n_groups} equal groups")
+    assert q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and out.is_contiguous() and out.shape[1] == n_heads * head_dim
+    assert q.shape[0] >= n_seqs and q.stride(-1) == 1
+    assert kv_lens.dtype == page_table.dtype == shared_pages.dtype == torch.int32
+    assert kv_lens.is_contiguous() and page_table.is_contiguous() and shared_pages.is_contiguous()
+    assert kv_lens.numel() == n_seqs and page_table.shape[0] == n_seqs
+    assert tuple(k_pool.shape[1:]) == (n_kv_heads, PAGE_TOKENS, head_dim) and k_pool.is_contiguous()
+    assert tuple(v_pool.shape[1:]) == (n_kv_heads, head_dim, PAGE_TOKENS) and v_pool.is_contiguous()
+    B = n_seqs // n_groups
+    floats, ints = _beams_numbers(n_groups, B, n_heads, n_kv_heads, head_dim, max(1, n_parts))
+    if scratch is None or scratch.numel() < floats:
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+    assert scratch.dtype == torch.float32 and scratch.is_contiguous()
+    assert plan is None or (plan.dtype == torch.int32 and plan.is_contiguous() and plan.numel() >= ints)
+    return n_groups, B, scratch
 
 
 def attention_decode_beams(q: torch.Tensor, q_row_stride: int, out: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor,
@@ -1289,32 +1341,34 @@ def attention_decode_beams(q: torch.Tensor, q_row_stride: int, out: torch.Tensor
     sequences g B .. (g + 1) B - 1, and the first shared_pages[g] entries of their rows of the page table are the same (int32 [groups]; pages
     that are not full for all of the group's sequences count as each one's own).  ``n_parts``: see ``attention_beams_parts``.  ``plan``: what
     ``attention_beams_plan`` made of the same lengths, shared pages, heads, window and width of the page table."""
-    _here(plan, q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, scratch)
-    n_seqs, n_groups = out.shape[0], shared_pages.numel()
-    if not attention_beams_supported(q.dtype, n_heads, n_kv_heads, head_dim):
-        raise KernelError(f"attention_decode_beams: {n_heads} heads on {n_kv_heads} of {head_dim} in {q.dtype}")
-    if n_groups == 0 or n_seqs % n_groups:
-        raise KernelError(f"{n_seqs} sequences do not make {n_groups} equal groups")
-    assert q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and out.is_contiguous() and out.shape[1] == n_heads * head_dim
-    assert q.stride(-1) == 1 and q_row_stride >= n_heads * head_dim
-    for t in (kv_lens, page_table, shared_pages):
-        assert t.dtype == torch.int32 and t.is_contiguous()
-    assert kv_lens.numel() == n_seqs and page_table.shape[0] == n_seqs
-    assert tuple(k_pool.shape[1:]) == (n_kv_heads, PAGE_TOKENS, head_dim) and k_pool.is_contiguous()
-    assert tuple(v_pool.shape[1:]) == (n_kv_heads, head_dim, PAGE_TOKENS) and v_pool.is_contiguous()
-    if n_seqs == 0:
+    if out.shape[0] == 0 and shared_pages.numel():
         return
-    B = n_seqs // n_groups
-    need_fn = library("attention_beams").b200_attention_beams_scratch_floats
-    need_fn.argtypes, need_fn.restype = [c_int] * 6, ctypes.c_longlong
-    need = int(need_fn(n_groups, B, n_heads, n_kv_heads, head_dim, n_parts))
-    if scratch is None or scratch.numel() < need:
-        scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-    assert scratch.dtype == torch.float32 and scratch.is_contiguous()
+    G, B, scratch = _beams_checked(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan)
+    assert q_row_stride >= n_heads * head_dim
     _check(_fn("b200_attention_beams")(
         q.data_ptr(), q_row_stride, out.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), page_table.shape[1], shared_pages.data_ptr(),
-        k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), n_groups, B, n_heads, n_kv_heads, head_dim, int(window),
+        k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), G, B, n_heads, n_kv_heads, head_dim, int(window),
         n_parts, dtype_code(q.dtype), plan.data_ptr() if plan is not None else None, _stream()), "attention_decode_beams")
+
+
+def attention_decode_beams_rope(qkv: torch.Tensor, out: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor,
+                                shared_pages: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, inv_freq: torch.Tensor, n_heads: int,
+                                n_kv_heads: int, head_dim: int, pairing: int, window: int, n_parts: int, write_cache: bool = True,
+                                scratch: torch.Tensor | None = None, *, plan: torch.Tensor | None = None) -> None:
+    """``attention_decode_beams`` that rotates the step's queries itself and, with ``write_cache``, stores the step's rotated keys and its values
+    at positions kv_lens - 1 (pages that no other sequence holds).  bfloat16; ``qkv``: the raw projections [n_seqs, (n_heads +
+    2 n_kv_heads) head_dim] (left untouched).  A ``plan`` is one made with the same ``writes_cache``."""
+    if out.shape[0] == 0 and shared_pages.numel():
+        return
+    _here(inv_freq)
+    G, B, scratch = _beams_checked(qkv, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan)
+    assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim
+    assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.numel() == head_dim // 2
+    _check(_fn("b200_attention_beams_rope")(
+        qkv.data_ptr(), qkv.shape[1], out.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), page_table.shape[1], shared_pages.data_ptr(),
+        k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), G, B, n_heads, n_kv_heads, head_dim, int(window),
+        n_parts, plan.data_ptr() if plan is not None else None, inv_freq.data_ptr(), pairing, 1 if write_cache else 0, _stream()),
+        "attention_decode_beams_rope")
 
 
 # --------------------------------------------------------------------------- several residual streams

@@ -446,3 +446,42 @@ def test_attention_of_groups_refuses():
     groups.H = 34
     with pytest.raises(ops.KernelError, match="34 heads on 2"):
         groups.run(parts=1)
+
+
+@pytest.mark.parametrize("pairing", [0, 1])
+@pytest.mark.parametrize("write_cache", [True, False])
+@pytest.mark.parametrize("shared, lens, H, KVH, D, window", [
+    ([0], [1, 1], 4, 2, 64, 0), ([1], [65, 66, 128], 8, 2, 64, 0), ([3, 0], [200, 256, 193, 5, 64, 1], 8, 8, 128, 0), ([5], [330] * 40, 6, 2, 32, 0),
+    ([2, 1], [150, 192, 129, 130, 180, 70, 91, 65, 128, 67], 16, 1, 96, 0), ([6, 2], [400, 450, 385, 130, 129, 192], 8, 2, 64, 100),
+    ([17, 4], [1100] * 4 + [300, 257, 320, 260], 32, 8, 64, 0),
+])
+def test_fused_rotation_and_cache_write(shared, lens, H, KVH, D, window, write_cache, pairing):
+    """The same bits as rotation and cache write in a kernel of their own and the attention behind it, in the cache too; and the same
+    result from a plan made beforehand."""
+    B = len(lens)
+    parts = ops.attention_beams_parts(len(shared), B // len(shared), H, KVH, D, 64 * 20, torch.bfloat16, "cuda")
+    one, two = (Groups(shared, lens, H, KVH, D, torch.bfloat16, seed=len(lens)) for _ in range(2))
+    qkv = (torch.randn(B, (H + 2 * KVH) * D, generator=torch.Generator().manual_seed(3)) * 1.4).to(torch.bfloat16).cuda()
+    inv_freq = (10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().cuda()
+    rotated = qkv.clone()
+    ops.rope_cache_write(rotated, one.lens - 1, torch.arange(B, dtype=torch.int32, device="cuda"), one.table, inv_freq, one.k, one.v, H, KVH, D, D,
+                         pairing, write_cache=write_cache)
+    want, got, again = (torch.empty(B, H * D, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    # (shared pages that reach the new position are refused to be shared by the fused form alone: compared on what is left)
+    fewer = torch.tensor([min(s, min(lens[i * (B // len(shared)):(i + 1) * (B // len(shared))]) - 1 >> 6) for i, s in enumerate(shared)],
+                         dtype=torch.int32, device="cuda")
+    ops.attention_decode_beams(rotated, rotated.shape[1], want, one.lens, one.table, fewer, one.k, one.v, H, KVH, D, window, parts)
+    raw = qkv.clone()
+    call = lambda out, plan: ops.attention_decode_beams_rope(raw, out, two.lens, two.table, two.shared if write_cache else fewer, two.k, two.v, inv_freq, H,
+                                                             KVH, D, pairing, window, parts, write_cache, plan=plan)
+    call(got, None)
+    assert torch.equal(raw, qkv) and torch.isfinite(want).all()
+    assert torch.equal(one.k.view(torch.int16), two.k.view(torch.int16)) and torch.equal(one.v.view(torch.int16), two.v.view(torch.int16))
+    assert torch.equal(got, want)
+    plan = ops.attention_beams_plan(two.lens, two.shared if write_cache else fewer, two.width, H, KVH, window, writes_cache=write_cache)
+    call(again, plan)
+    assert torch.equal(again, want)
+    plain_plan = ops.attention_beams_plan(one.lens, fewer, one.width, H, KVH, window)
+    again.zero_()
+    ops.attention_decode_beams(rotated, rotated.shape[1], again, one.lens, one.table, fewer, one.k, one.v, H, KVH, D, window, parts, plan=plain_plan)
+    assert torch.equal(again, want)
