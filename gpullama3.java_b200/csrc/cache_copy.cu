@@ -7,88 +7,140 @@
 // several launches.  Sources are never destinations and no destination comes twice (the caller sees to it), so the order of
 // CTAs does not matter.
 //
-// What is copied lies in slabs: of a page and entry, a head's keys are one run of bytes (positions are rows), its values are
-// head_dim rows of 64 positions of which the first n are taken; a state is cut into runs of 16 KB.  A CTA takes one slab of one
-// source, four 16-byte loads a thread at a time.  Bound by HBM.
+// Pages: a CTA takes a head of an entry of one source.  Its keys are one run of bytes (positions follow one another), its values head_dim rows of
+// 64 positions of which the first n are taken; 16 bytes an access, four of the keys and four of the values a thread asked for before the first
+// is stored.  States: a CTA takes 2,048 accesses (of the widest that the addresses allow) of one state, eight a thread.  Bound by HBM, and
+// where pages are not full by the sectors that rows of values end in: they are read to be written.
 #include "common.cuh"
 
 namespace b200 {
 
-constexpr int kCopyThreads = 128;
-constexpr int kCopyAtOnce = 4;
+constexpr int kCopyThreads = 256;
+constexpr int kPageAtOnce = 2, kTailAtOnce = 2, kSlotAtOnce = 8;
 constexpr int kMaxSources = 96, kMaxDestinations = 256;     // of one launch (an argument holds 4 KB)
-constexpr int kStateSlab = 16384;
 
 struct Moves {
     int source[kMaxSources], positions[kMaxSources], first[kMaxSources + 1], destination[kMaxDestinations];
 };
 
-struct Slabs {              // a kind of storage: [entry][index][slab of rows]
-    unsigned char* base;
-    long long entry_stride, index_stride, slab_stride, row_stride;      // bytes
-    long long bytes;        // of an index and entry (states: the last slab is cut there); 0: slabs are whole
-    int per_index;          // slabs of an index and entry
-    int rows;               // of a slab
-    int position_bytes;     // of a row and position
+struct Pages {
+    unsigned char* keys;
+    unsigned char* values;
+    long long entry, page;      // bytes between entries and between pages
+    int head, kv_heads;         // bytes of a head's keys or values, heads
+    int head_dim, element;
 };
 
-// W: bytes of an access.  What remains of a row behind its whole accesses is blended into the destination's bytes.
-template <typename W>
-__global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_constant__ Moves moves, const __grid_constant__ Slabs a,
-                                                                 const __grid_constant__ Slabs b, int slabs_a) {
+// the first `bytes` (even, at most 16) of `w`, the others of `old`
+__device__ __forceinline__ uint4 blended(const uint4& w, const uint4& old, int bytes) {
+    const unsigned a[4] = {w.x, w.y, w.z, w.w}, b[4] = {old.x, old.y, old.z, old.w};
+    unsigned r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int left = bytes - 4 * i;
+        r[i] = left >= 4 ? a[i] : left == 2 ? (a[i] & 0xffffu) | (b[i] & 0xffff0000u) : b[i];
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+__global__ void __launch_bounds__(kCopyThreads, 4) copy_pages_kernel(const __grid_constant__ Moves moves, const __grid_constant__ Pages p) {
     pdl_launch_dependents();
     pdl_wait();
-    const bool second = (int)blockIdx.x >= slabs_a;
-    const Slabs& s = second ? b : a;
-    const int at = second ? blockIdx.x - slabs_a : blockIdx.x;
-    const int entry = at / s.per_index, slab = at % s.per_index;
-    const int group = blockIdx.y;
-    const size_t offset = (size_t)entry * s.entry_stride + (size_t)slab * s.slab_stride;
-    const unsigned char* from = s.base + offset + (size_t)moves.source[group] * s.index_stride;
-    long long row_bytes = (long long)moves.positions[group] * s.position_bytes;
-    if (s.bytes) row_bytes = min(row_bytes, s.bytes - (long long)slab * s.slab_stride);
-    const int per_row = (int)((row_bytes + sizeof(W) - 1) / sizeof(W)), n = per_row * s.rows;
-    const int rest = (int)(row_bytes % sizeof(W));       // bytes of a row's last access, if it is not whole
-    const int first = moves.first[group], last = moves.first[group + 1];
-    for (int i0 = threadIdx.x; i0 < n; i0 += kCopyThreads * kCopyAtOnce) {
-        W v[kCopyAtOnce];
-        size_t where[kCopyAtOnce];
-        bool cut[kCopyAtOnce];
+    const int group = blockIdx.y, entry = blockIdx.x / p.kv_heads, head = blockIdx.x - entry * p.kv_heads, positions = moves.positions[group];
+    const size_t at = (size_t)entry * p.entry + (size_t)head * p.head;
+    const int row_bytes = positions * p.element, pitch = kPageTokens * p.element, first = moves.first[group], last = moves.first[group + 1];
+    const unsigned char* from_k = p.keys + at + (size_t)moves.source[group] * p.page;
+    const unsigned char* from_v = p.values + at + (size_t)moves.source[group] * p.page;
+    // What a row of values has in its last sector, if that is not full.  The sector is stored whole, with what the destination has behind the last
+    // position: a store of a part of a sector costs HBM a read and a write of its own (40 pages of 31 positions took 103 us, of 32 53 us).
+    const int tail = row_bytes % 32, tail_at = row_bytes - tail, n_tails = tail ? (last - first) * p.head_dim * 2 : 0;
+    uint4 old[kTailAtOnce], fresh[kTailAtOnce];
+    auto tail_place = [&](int i) {          // piece i of the tails: destinations, rows, two halves
+        const int d = i / (2 * p.head_dim), r = i - d * 2 * p.head_dim;
+        return make_int2(first + d, (r >> 1) * pitch + tail_at + (r & 1) * 16);
+    };
+    auto ask_tails = [&](int i0) {
 #pragma unroll
-        for (int u = 0; u < kCopyAtOnce; ++u) {
-            const int i = i0 + u * kCopyThreads, row = i / per_row, c = i - row * per_row;
-            where[u] = (size_t)row * s.row_stride + (size_t)c * sizeof(W);
-            cut[u] = rest != 0 && c == per_row - 1;
-            if (i < n) v[u] = *reinterpret_cast<const W*>(from + where[u]);
+        for (int u = 0; u < kTailAtOnce; ++u) {
+            const int i = i0 + u * kCopyThreads;
+            if (i >= n_tails) continue;
+            const int2 t = tail_place(i);
+            old[u] = *reinterpret_cast<const uint4*>(p.values + at + (size_t)moves.destination[t.x] * p.page + t.y);
+            fresh[u] = *reinterpret_cast<const uint4*>(from_v + t.y);
+        }
+    };
+    ask_tails(threadIdx.x);
+    const int n_keys = positions * p.head_dim * p.element / 16;                     // (a position's keys are whole pieces)
+    const int per = row_bytes / 32 * 2, n_values = per * p.head_dim;
+    const unsigned magic = per > 0 ? (unsigned)(((1ull << 32) + per - 1) / per) : 0u;   // (exact: pieces are below 2^16, per is 2 to 16)
+    for (int i0 = threadIdx.x; i0 < max(n_keys, n_values); i0 += kCopyThreads * kPageAtOnce) {
+        uint4 k[kPageAtOnce], v[kPageAtOnce];
+        int place[kPageAtOnce];
+#pragma unroll
+        for (int u = 0; u < kPageAtOnce; ++u) {
+            const int i = i0 + u * kCopyThreads, row = (int)__umulhi((unsigned)i, magic);
+            place[u] = row * pitch + (i - row * per) * 16;
+            if (i < n_keys) k[u] = *reinterpret_cast<const uint4*>(from_k + i * 16);
+            if (i < n_values) v[u] = *reinterpret_cast<const uint4*>(from_v + place[u]);
         }
         for (int d = first; d < last; ++d) {
-            unsigned char* to = s.base + offset + (size_t)moves.destination[d] * s.index_stride;
+            const size_t to = at + (size_t)moves.destination[d] * p.page;
 #pragma unroll
-            for (int u = 0; u < kCopyAtOnce; ++u) {
-                if (i0 + u * kCopyThreads >= n) continue;
-                if (!cut[u]) {
-                    *reinterpret_cast<W*>(to + where[u]) = v[u];
-                } else {        // (elements are of two bytes or four: so is what remains)
-                    const unsigned short* halves = reinterpret_cast<const unsigned short*>(&v[u]);
-#pragma unroll
-                    for (int k = 0; k < (int)sizeof(W) / 2; ++k)
-                        if (2 * k < rest) reinterpret_cast<unsigned short*>(to + where[u])[k] = halves[k];
-                }
+            for (int u = 0; u < kPageAtOnce; ++u) {
+                const int i = i0 + u * kCopyThreads;
+                if (i < n_keys) *reinterpret_cast<uint4*>(p.keys + to + i * 16) = k[u];
+                if (i < n_values) *reinterpret_cast<uint4*>(p.values + to + place[u]) = v[u];
             }
+        }
+    }
+    for (int i0 = threadIdx.x; i0 < n_tails; i0 += kCopyThreads * kTailAtOnce) {
+        if (i0 >= kCopyThreads * kTailAtOnce) ask_tails(i0);
+#pragma unroll
+        for (int u = 0; u < kTailAtOnce; ++u) {
+            const int i = i0 + u * kCopyThreads;
+            if (i >= n_tails) continue;
+            const int2 t = tail_place(i);
+            *reinterpret_cast<uint4*>(p.values + at + (size_t)moves.destination[t.x] * p.page + t.y) =
+                blended(fresh[u], old[u], min(16, max(0, tail - (i & 1) * 16)));
         }
     }
 }
 
-static int launch_copies(const int* sources, const int* positions, const int* firsts, int n_sources, const int* destinations, const Slabs& a,
-                         const Slabs& b, int slabs_a, int slabs_b, int width, cudaStream_t stream) {
+struct Slots {
+    unsigned char* data;
+    long long entry, slot, pieces;      // bytes between entries and between slots; accesses of a state
+    int blocks;                         // CTAs of a state
+};
+
+template <typename W>
+__global__ void __launch_bounds__(kCopyThreads) copy_slots_kernel(const __grid_constant__ Moves moves, const __grid_constant__ Slots s) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int entry = blockIdx.x / s.blocks, block = blockIdx.x - entry * s.blocks, group = blockIdx.y;
+    const long long i0 = (long long)block * (kCopyThreads * kSlotAtOnce) + threadIdx.x;
+    unsigned char* at = s.data + (size_t)entry * s.entry;
+    const W* from = reinterpret_cast<const W*>(at + (size_t)moves.source[group] * s.slot) + i0;
+    W v[kSlotAtOnce];
+#pragma unroll
+    for (int u = 0; u < kSlotAtOnce; ++u) if (i0 + u * kCopyThreads < s.pieces) v[u] = from[u * kCopyThreads];
+    for (int d = moves.first[group]; d < moves.first[group + 1]; ++d) {
+        W* to = reinterpret_cast<W*>(at + (size_t)moves.destination[d] * s.slot) + i0;
+#pragma unroll
+        for (int u = 0; u < kSlotAtOnce; ++u) if (i0 + u * kCopyThreads < s.pieces) to[u * kCopyThreads] = v[u];
+    }
+}
+
+// As many launches as the lists need: `launch(moves, number of sources)` each.
+template <typename Launch>
+static int in_arguments(const int* sources, const int* positions, const int* firsts, int n_sources, const int* destinations, Launch launch) {
     Moves m;
     int at = 0, done = 0;       // source and destination reached
     while (at < n_sources) {
         int n = 0, count = 0;
         while (at < n_sources && n < kMaxSources && count < kMaxDestinations) {
-            const int take = min(firsts[at + 1] - done, kMaxDestinations - count);
+            const int left = firsts[at + 1] - done, room = kMaxDestinations - count, take = left < room ? left : room;
             m.source[n] = sources[at];
-            m.positions[n] = positions ? positions[at] : 1;     // (a state's slab is its one position)
+            m.positions[n] = positions ? positions[at] : 0;
             m.first[n] = count;
             for (int i = 0; i < take; ++i) m.destination[count + i] = destinations[done + i];
             count += take;
@@ -97,15 +149,7 @@ static int launch_copies(const int* sources, const int* positions, const int* fi
             if (done == firsts[at + 1]) ++at;
         }
         m.first[n] = count;
-        const dim3 grid(slabs_a + slabs_b, n), block(kCopyThreads);
-        int st;
-        switch (width) {
-            case 16: st = launch_pdl(cache_copy_kernel<uint4>, grid, block, 0, stream, m, a, b, slabs_a); break;
-            case 8: st = launch_pdl(cache_copy_kernel<uint2>, grid, block, 0, stream, m, a, b, slabs_a); break;
-            case 4: st = launch_pdl(cache_copy_kernel<unsigned int>, grid, block, 0, stream, m, a, b, slabs_a); break;
-            case 2: st = launch_pdl(cache_copy_kernel<unsigned short>, grid, block, 0, stream, m, a, b, slabs_a); break;
-            default: st = launch_pdl(cache_copy_kernel<unsigned char>, grid, block, 0, stream, m, a, b, slabs_a); break;
-        }
+        const int st = launch(m, n);
         if (st != 0) return st;
     }
     return 0;
@@ -124,11 +168,12 @@ extern "C" int b200_copy_pages(void* keys, void* values, long long entry_element
     if (n_kv_heads < 1 || head_dim < 1 || (element != 2 && element != 4)) return kErrBadArgument;
     if ((head_dim * element) % 16 != 0 || (entry_elements * element) % 16 != 0 || (((uintptr_t)keys | (uintptr_t)values) & 15) != 0)
         return kErrUnsupportedSize;
-    const long long head = (long long)kPageTokens * head_dim * element, page = head * n_kv_heads, entry = entry_elements * element;
-    const Slabs k{(unsigned char*)keys, entry, page, head, head, 0, n_kv_heads, 1, head_dim * element};
-    const Slabs v{(unsigned char*)values, entry, page, head, kPageTokens * element, 0, n_kv_heads, head_dim, element};
-    const int slabs = n_entries * n_kv_heads;
-    return launch_copies(sources, positions, firsts, n_sources, destinations, k, v, slabs, slabs, 16, stream);
+    if ((long long)n_entries * n_kv_heads > 0x7fffffffll || head_dim > 1024) return kErrUnsupportedSize;
+    const long long head = (long long)kPageTokens * head_dim * element;
+    const Pages p{(unsigned char*)keys, (unsigned char*)values, entry_elements * element, head * n_kv_heads, (int)head, n_kv_heads, head_dim, element};
+    return in_arguments(sources, positions, firsts, n_sources, destinations, [&](const Moves& m, int n) {
+        return launch_pdl(copy_pages_kernel, dim3(n_entries * n_kv_heads, n), dim3(kCopyThreads), 0, stream, m, p);
+    });
 }
 
 // data [entry][slot] of `bytes` bytes each, slots `slot_stride` bytes apart, entries `entry_stride`; lists as above, without positions.
@@ -139,8 +184,17 @@ extern "C" int b200_copy_slots(void* data, long long entry_stride, long long slo
     const unsigned long long all = (unsigned long long)(uintptr_t)data | entry_stride | slot_stride | bytes;
     int width = 16;
     while (all % width) width /= 2;
-    const long long per_index = (bytes + kStateSlab - 1) / kStateSlab;
-    if (per_index * n_entries > 0x7fffffffll) return kErrUnsupportedSize;
-    const Slabs s{(unsigned char*)data, entry_stride, slot_stride, kStateSlab, kStateSlab, bytes, (int)per_index, 1, kStateSlab};
-    return launch_copies(sources, nullptr, firsts, n_sources, destinations, s, s, (int)per_index * n_entries, 0, width, stream);
+    const long long pieces = bytes / width, blocks = (pieces + kCopyThreads * kSlotAtOnce - 1) / (kCopyThreads * kSlotAtOnce);
+    if (blocks * n_entries > 0x7fffffffll) return kErrUnsupportedSize;
+    const Slots s{(unsigned char*)data, entry_stride, slot_stride, pieces, (int)blocks};
+    return in_arguments(sources, nullptr, firsts, n_sources, destinations, [&](const Moves& m, int n) {
+        const dim3 grid((unsigned)(blocks * n_entries), n), block(kCopyThreads);
+        switch (width) {
+            case 16: return launch_pdl(copy_slots_kernel<uint4>, grid, block, 0, stream, m, s);
+            case 8: return launch_pdl(copy_slots_kernel<uint2>, grid, block, 0, stream, m, s);
+            case 4: return launch_pdl(copy_slots_kernel<unsigned int>, grid, block, 0, stream, m, s);
+            case 2: return launch_pdl(copy_slots_kernel<unsigned short>, grid, block, 0, stream, m, s);
+            default: return launch_pdl(copy_slots_kernel<unsigned char>, grid, block, 0, stream, m, s);
+        }
+    });
 }

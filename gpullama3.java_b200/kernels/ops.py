@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from ctypes import c_float, c_int, c_void_p
 
 import torch
@@ -1153,6 +1154,9 @@ def beam_select_takes(beams: int, keep: int) -> bool:
     return 1 <= beams <= 1024 and 1 <= keep <= BEAM_MAX_KEEP
 
 
+_beam_select_bytes: dict = {}
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, out_scores: torch.Tensor, out_beams: torch.Tensor, out_tokens: torch.Tensor,
                 scratch: torch.Tensor | None = None) -> None:
     """The best continuations of each request's beams, best first.  ``logits`` float32 [G * B, V] (rows may be apart); ``scores`` float32
@@ -1164,79 +1168,95 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, out_scores: torch.Te
     _here(logits, scores, out_scores, out_beams, out_tokens, scratch)
     if scores.dim() != 2 or out_scores.dim() != 2 or logits.dim() != 2:
         raise KernelError("beam_select takes logits [G * B, V], scores [G, B] and results [G, n]")
-    (G, B), n = scores.shape, out_scores.shape[1]
+    (G, B), n, (rows, V) = scores.shape, out_scores.shape[1], logits.shape
     assert logits.dtype == scores.dtype == out_scores.dtype == torch.float32 and out_beams.dtype == out_tokens.dtype == torch.int32
-    assert logits.shape[0] == G * B and logits.shape[1] >= 1 and (logits.stride(1) == 1 or logits.shape[1] == 1)
-    assert scores.is_contiguous() and all(t.is_contiguous() and tuple(t.shape) == (G, n) for t in (out_scores, out_beams, out_tokens))
-    if not beam_select_takes(B, n) or G * B > 65535:
+    ld, step = logits.stride()
+    assert rows == G * B and V >= 1 and (step == 1 or V == 1) and (ld >= V or rows <= 1)
+    assert out_scores.shape[0] == G and out_beams.shape == out_tokens.shape == out_scores.shape
+    assert scores.is_contiguous() and out_scores.is_contiguous() and out_beams.is_contiguous() and out_tokens.is_contiguous()
+    if not beam_select_takes(B, n) or rows > 65535:
         raise KernelError(f"beam_select: {G} requests of {B} beams, {n} continuations each (at most 65,535 rows, 1,024 beams, "
                           f"{BEAM_MAX_KEEP} continuations)")
     if G == 0:
         return
-    ld = logits.stride(0) if G * B > 1 else logits.shape[1]
-    need_fn = library("beam_select").b200_beam_select_scratch_bytes
-    need_fn.argtypes, need_fn.restype = [c_int, c_int, c_int], ctypes.c_longlong
-    need = int(need_fn(G * B, logits.shape[1], n))
+    key = (rows, V, n, logits.get_device())     # (how rows are cut depends on the device's SMs)
+    need = _beam_select_bytes.get(key)
+    if need is None:
+        size = library("beam_select").b200_beam_select_scratch_bytes
+        size.argtypes, size.restype = [c_int, c_int, c_int], ctypes.c_longlong
+        if len(_beam_select_bytes) > 1000:
+            _beam_select_bytes.clear()
+        need = _beam_select_bytes[key] = int(size(rows, V, n))
     if scratch is None or scratch.numel() < need:
         scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
     assert scratch.dtype == torch.uint8 and scratch.is_contiguous() and scratch.data_ptr() % 16 == 0
-    _check(_fn("b200_beam_select")(logits.data_ptr(), ld, scores.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(),
-                                   out_tokens.data_ptr(), scratch.data_ptr(), scratch.numel(), G, B, logits.shape[1], n, _stream()),
+    _check(_fn("b200_beam_select")(logits.data_ptr(), ld if rows > 1 else V, scores.data_ptr(), out_scores.data_ptr(), out_beams.data_ptr(),
+                                   out_tokens.data_ptr(), scratch.data_ptr(), scratch.numel(), G, B, V, n, _stream()),
            "beam_select")
 
 
 def copy_groups(moves, n: int):
     """Moves (source, destination, ...) by source, as the copy kernels take them: int32 arrays of the sources, of where each one's
-    destinations begin, and of the destinations, with the first move of each source.  Refuses numbers outside [0, n), a destination
-    that comes twice or is a source too."""
+    destinations begin, and of the destinations.  Refuses numbers outside [0, n), a destination that comes twice or is a source too."""
     by_source: dict = {}
     seen = set()
     for m in moves:
-        s, d = int(m[0]), int(m[1])
-        if not (0 <= s < n and 0 <= d < n):
-            raise KernelError(f"a move from {s} to {d}: there are {n}")
+        d = m[1]
         if d in seen:
             raise KernelError(f"{d} is the destination of two moves")
         seen.add(d)
-        by_source.setdefault(s, []).append(m)
-    for s in by_source:
-        if s in seen:
-            raise KernelError(f"{s} is a source and a destination")
-    firsts = [0]
+        by_source.setdefault(m[0], []).append(d)
+    if seen:
+        for numbers in (seen, by_source):
+            if min(numbers) < 0 or max(numbers) >= n:
+                raise KernelError(f"moves from {sorted(by_source)} to {sorted(seen)}: there are {n}")
+        if not seen.isdisjoint(by_source):
+            raise KernelError(f"{min(seen.intersection(by_source))} is a source and a destination")
+    firsts, destinations = [0], []
     for group in by_source.values():
-        firsts.append(firsts[-1] + len(group))
-    ints = lambda xs: (c_int * max(1, len(xs)))(*xs)
-    return (ints(list(by_source)), ints(firsts), ints([int(m[1]) for group in by_source.values() for m in group]),
-            [group for group in by_source.values()])
+        destinations += group
+        firsts.append(len(destinations))
+    return array("i", by_source), array("i", firsts), array("i", destinations)
+
+
+def _rows_together(t: torch.Tensor, first: int) -> bool:
+    """Whether the dimensions of ``t`` from ``first`` on lie as one run."""
+    want = 1
+    for size, stride in zip(reversed(t.shape[first:]), reversed(t.stride()[first:])):
+        if size != 1 and stride != want:
+            return False
+        want *= size
+    return True
 
 
 def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, moves) -> None:
     """Copies the first positions of cache pages: for every (source, destination, positions) of ``moves`` positions 0 .. positions - 1 of
     page ``source`` go to page ``destination``, in every entry and head; the destination's other positions stay.  Pools
     [entries, pages, kv_heads, 64, head_dim] and [entries, pages, kv_heads, head_dim, 64], or of one entry without the first dimension.  A page
-    may be the source of several moves (read once; they must ask for as many positions), the destination of one, and not both."""
+    may be the source of several moves (read once; they must ask for as many positions), the destination of one, and not both.  The
+    moves travel with the launch: a recorded one repeats the same."""
     _here(k_pool, v_pool)
     if k_pool.dim() == 4:
         k_pool, v_pool = k_pool.unsqueeze(0), v_pool.unsqueeze(0)
     E, P, H, T, D = k_pool.shape
     assert k_pool.dtype == v_pool.dtype and T == PAGE_TOKENS and tuple(v_pool.shape) == (E, P, H, D, PAGE_TOKENS)
     dtype_code(k_pool.dtype)
-    assert k_pool[0].is_contiguous() and v_pool[0].is_contiguous() and (E == 1 or k_pool.stride(0) == v_pool.stride(0))
-    sources, firsts, destinations, groups = copy_groups(moves, P)
-    positions = []
-    for group in groups:
-        n = int(group[0][2])
-        if not 0 <= n <= PAGE_TOKENS:
-            raise KernelError(f"{n} positions of a page of {PAGE_TOKENS}")
-        if any(int(m[2]) != n for m in group):
-            raise KernelError(f"page {group[0][0]} is copied with two numbers of positions")
-        positions.append(n)
-    if not groups:
+    assert _rows_together(k_pool, 1) and _rows_together(v_pool, 1)
+    entry = k_pool.stride(0) if E > 1 else P * H * T * D
+    assert E == 1 or (v_pool.stride(0) == entry and entry >= P * H * T * D)
+    sources, firsts, destinations = copy_groups(moves, P)
+    positions: dict = {}
+    for m in moves:
+        if positions.setdefault(m[0], m[2]) != m[2]:
+            raise KernelError(f"page {m[0]} is copied with two numbers of positions")
+    if not positions:
         return
-    counts = (c_int * len(positions))(*positions)
-    _check(_fn("b200_copy_pages")(k_pool.data_ptr(), v_pool.data_ptr(), k_pool.stride(0) if E > 1 else P * H * T * D, E, H, D,
-                                  k_pool.element_size(), ctypes.addressof(sources), ctypes.addressof(counts), ctypes.addressof(firsts),
-                                  len(groups), ctypes.addressof(destinations), _stream()), "copy_pages")
+    if min(positions.values()) < 0 or max(positions.values()) > PAGE_TOKENS:
+        raise KernelError(f"{sorted(positions.values())} positions of pages of {PAGE_TOKENS}")
+    counts = array("i", positions.values())
+    at = lambda a: a.buffer_info()[0]
+    _check(_fn("b200_copy_pages")(k_pool.data_ptr(), v_pool.data_ptr(), entry, E, H, D, k_pool.element_size(), at(sources), at(counts), at(firsts),
+                                  len(sources), at(destinations), _stream()), "copy_pages")
 
 
 def copy_slots(data: torch.Tensor, moves) -> None:
@@ -1245,18 +1265,19 @@ def copy_slots(data: torch.Tensor, moves) -> None:
     _here(data)
     if data.dim() < 2:
         raise KernelError("copy_slots takes data [entries, slots, ...]")
-    sources, firsts, destinations, groups = copy_groups(moves, data.shape[1])
-    if not groups or data.numel() == 0:
+    E, S = data.shape[:2]
+    sources, firsts, destinations = copy_groups(moves, S)
+    if not sources or data.numel() == 0:
         return
-    assert data[0, 0].is_contiguous()
-    size = data.element_size()
-    n_bytes = data[0, 0].numel() * size
-    # (a stride of 0, or one smaller than a state, would make two of them one)
-    assert data.shape[1] == 1 or data.stride(1) * size >= n_bytes
-    assert data.shape[0] == 1 or data.stride(0) * size >= n_bytes
-    _check(_fn("b200_copy_slots")(data.data_ptr(), data.stride(0) * size if data.shape[0] > 1 else 0, data.stride(1) * size, n_bytes,
-                                  data.shape[0], ctypes.addressof(sources), ctypes.addressof(firsts), len(groups),
-                                  ctypes.addressof(destinations), _stream()), "copy_slots")
+    assert _rows_together(data, 2)
+    size, n = data.element_size(), data.numel() // (E * S)
+    # (states that overlap would be written while they are read)
+    slot, entry = (data.stride(1) if S > 1 else n), (data.stride(0) if E > 1 else S * n)
+    assert slot >= n and (E == 1 or entry >= n)
+    assert E == 1 or S == 1 or entry >= (S - 1) * slot + n or slot >= (E - 1) * entry + n
+    at = lambda a: a.buffer_info()[0]
+    _check(_fn("b200_copy_slots")(data.data_ptr(), entry * size, slot * size, n * size, E, at(sources), at(firsts), len(sources),
+                                  at(destinations), _stream()), "copy_slots")
 
 
 def attention_beams_supported(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:

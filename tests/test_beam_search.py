@@ -408,8 +408,9 @@ def test_a_request_without_beams_that_count_is_over():
 
 
 def test_moves_are_grouped_by_source():
-    sources, firsts, destinations, groups = ops.copy_groups([(3, 1, 5), (0, 2, 7), (3, 4, 5)], 6)
-    assert list(sources) == [3, 0] and list(firsts) == [0, 2, 3] and list(destinations) == [1, 4, 2] and len(groups) == 2
+    sources, firsts, destinations = ops.copy_groups([(3, 1, 5), (0, 2, 7), (3, 4, 5)], 6)
+    assert list(sources) == [3, 0] and list(firsts) == [0, 2, 3] and list(destinations) == [1, 4, 2]
+    assert [list(a) for a in ops.copy_groups([], 6)] == [[], [0], []]
     for moves, what in [([(6, 0)], "there are 6"), ([(0, -1)], "there are 6"), ([(0, 1), (2, 1)], "two moves"), ([(0, 1), (1, 2)], "source and")]:
         with pytest.raises(ops.KernelError, match=what):
             ops.copy_groups(moves, 6)

@@ -241,7 +241,7 @@ def test_state_copies(dtype, shape):
 
 def test_copies_refuse():
     k, v = torch.zeros(1, 4, 1, 64, 16, device="cuda"), torch.zeros(1, 4, 1, 16, 64, device="cuda")
-    for moves, what in [([(0, 4, 1)], "there are 4"), ([(-1, 2, 1)], "there are 4"), ([(0, 1, 65)], "65 positions"), ([(0, 1, -1)], "-1 positions"),
+    for moves, what in [([(0, 4, 1)], "there are 4"), ([(-1, 2, 1)], "there are 4"), ([(0, 1, 65)], "65. positions"), ([(0, 1, -1)], "-1. positions"),
                         ([(0, 1, 3), (2, 1, 3)], "two moves"), ([(0, 1, 3), (1, 2, 3)], "source and a destination"), ([(2, 2, 3)], "source and a destination"),
                         ([(0, 1, 3), (0, 2, 4)], "two numbers")]:
         with pytest.raises(ops.KernelError, match=what):

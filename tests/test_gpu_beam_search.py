@@ -126,14 +126,14 @@ WIDE = {"architectures": ["LlamaForCausalLM"], "num_hidden_layers": 2, "hidden_s
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("graphs", [True, False])
 def test_search_over_long_shared_prompts(session_tmp, dtype, graphs):
-    """Several full pages shared by the beams, in recorded steps and in steps launched one by one: the attention of groups runs."""
+    """Many full pages shared by the beams, in recorded steps and in steps launched one by one: the attention of groups runs."""
     from gpullama3.java_b200.engine.api import Engine
     from gpullama3.java_b200.kernels import ops
 
     d = make_model_dir(session_tmp, WIDE, seed=4, scale={"embed_tokens": 8.0, "lm_head": 4.0, "q_proj": 3.0, "k_proj": 3.0})
-    engine = Engine.from_folder(d, dtype=dtype, max_tokens=64 * 200, max_batch=16)
+    engine = Engine.from_folder(d, dtype=dtype, max_tokens=64 * 200, max_batch=20)
     engine.step_fn.use_graphs = graphs
-    prompts = random_prompts(3000, [700, 64, 333, 190], seed=6)
+    prompts = random_prompts(3000, [1100, 64, 333, 190, 961], seed=6)
     launches = lambda: sum(n for name, n in ops.launches_by_kernel().items() if name.startswith("attention_decode_beams"))
     before = launches()
     got = engine.beam_search(prompts, 4, 70, n_best=4, stop_ids=(), return_hypotheses=True)      # (beams fill pages of their own)
@@ -141,7 +141,7 @@ def test_search_over_long_shared_prompts(session_tmp, dtype, graphs):
     _check_hypotheses(engine, prompts, got, 2e-5 if dtype == "float32" else 4 * BF16_EPS)
     if not graphs:
         return
-    plain = Engine.from_folder(d, dtype=dtype, max_tokens=64 * 200, max_batch=16)
+    plain = Engine.from_folder(d, dtype=dtype, max_tokens=64 * 200, max_batch=20)
     plain.step_fn.use_graphs = False
     other = plain.beam_search(prompts, 4, 70, n_best=4, stop_ids=(), return_hypotheses=True)
     assert [h.tokens for hyps in other for h in hyps[:1]] == [h.tokens for hyps in got for h in hyps[:1]] or dtype == "bfloat16"
