@@ -26,7 +26,7 @@ constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamEach = 16;                           // logits of a thread at a time
 constexpr int kBeamTile = kBeamThreads * kBeamEach;
 constexpr int kBeamMaxKeep = 256;
-constexpr int kBeamLimit = 768;                         // most candidates of a list that is not cut down (3 keep)
+constexpr int kBeamLimit = 2 * kBeamMaxKeep + 64;       // most candidates of a list that is not cut down
 constexpr int kBeamList = kBeamLimit + kBeamTile;       // most that it holds
 constexpr int kMergeThreads = 512;
 constexpr int kMergeList = 1024;
@@ -72,7 +72,6 @@ __device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (
 struct RowsShared {
     u64 list[kBeamList];                // 36 KB
     int n;
-    unsigned best[kBeamThreads];        // the threads' maxima of the first tile
     float ref[kBeamWarps];
     double sum[kBeamWarps];
     int count[2][kBeamWarps];
@@ -107,6 +106,23 @@ __device__ __forceinline__ unsigned cut_down(RowsShared& sh, int keep) {
 #pragma unroll
     for (int w = 0; w < kBeamWarps; ++w) { high = max(high, sh.high[w]); low = min(low, sh.low[w]); }
     const int differing = 32 - __clz(high ^ low);
+    if (n <= kBeamThreads) {            // one candidate a thread: it stays in a register, and a barrier counts
+        const u64 key = tid < n ? sh.list[tid] : 0ull;
+        u64 least = differing == 32 ? 0ull : ((u64)high << 32) >> (32 + differing) << (32 + differing);
+        for (int bit = 31 + differing; bit >= 0; --bit) {
+            const u64 t = least | (1ull << bit);
+            const int reach = __syncthreads_count(key >= t);
+            if (reach >= keep) {
+                least = t;
+                if (reach <= keep + keep / 4) break;
+            }
+        }
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        if (key >= least && key != 0ull) sh.list[atomicAdd(&sh.n, 1)] = key;
+        __syncthreads();
+        return (unsigned)(least >> 32);
+    }
     u64 least = differing == 32 ? 0ull : ((u64)high << 32) >> (32 + differing) << (32 + differing);
     for (int bit = 31 + differing; bit >= 0; --bit) {
         const u64 t = least | (1ull << bit);
@@ -169,7 +185,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
             for (int e = 0; e < kBeamEach; ++e) x[e] = place(e) < n ? __ldg(x0 + place(e)) : -INFINITY;
         }
     };
-    const int limit = max(128, 3 * keep);
+    const int limit = max(128, 2 * keep + 64);
     float border = 0.f;         // what candidates reach
     float ref = -INFINITY;      // the thread's exponentials are relative to it
     double total = 0.0;
@@ -185,20 +201,12 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
 
         if (base == first) {
             // What about the keep-th largest of the threads' maxima reach, at least `keep` logits do, and few more.
-            const unsigned key = isnan(mine) ? 0u : rising_bits(mine);
-            sh.best[tid] = key;
-            const unsigned top = __reduce_max_sync(0xffffffffu, key);
+            const unsigned key = isnan(mine) ? 0u : rising_bits(mine), top = __reduce_max_sync(0xffffffffu, key);
             ref = top ? from_rising_bits(top) : -INFINITY;
-            __syncthreads();
-            unsigned best[kBeamThreads / 32], least = 0;
-#pragma unroll
-            for (int u = 0; u < kBeamThreads / 32; ++u) best[u] = sh.best[u * 32 + lane];
+            unsigned least = 0;
             for (int bit = 31; bit >= 0; --bit) {
                 const unsigned t = least | (1u << bit);
-                int n = 0;
-#pragma unroll
-                for (int u = 0; u < kBeamThreads / 32; ++u) n += best[u] >= t ? 1 : 0;
-                n = __reduce_add_sync(0xffffffffu, n);
+                const int n = __syncthreads_count(key >= t);
                 if (n >= keep) {
                     least = t;
                     if (n <= keep + keep / 4) break;
