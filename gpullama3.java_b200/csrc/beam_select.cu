@@ -530,7 +530,7 @@ extern "C" int b200_beam_select(const float* logits, long long ld, const float* 
     using namespace b200;
     if (n_groups <= 0) return 0;
     if (beams < 1 || vocab < 1 || keep < 1 || ld < vocab) return kErrBadArgument;
-    if (keep > kBeamMaxKeep || beams > 1024 || (long long)n_groups * beams > 65535) return kErrUnsupportedSize;
+    if (keep > kBeamMaxKeep || beams > 1024 || vocab > (1 << 30) || (long long)n_groups * beams > 65535) return kErrUnsupportedSize;
     const long long rows = (long long)n_groups * beams;
     const int tiles = tiles_of(rows, vocab), chunks = (vocab + tiles * kBeamTile - 1) / (tiles * kBeamTile);
     if (scratch_bytes < b200_beam_select_scratch_bytes((int)rows, vocab, keep)) return 10003;

@@ -1174,9 +1174,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, out_scores: torch.Te
     assert rows == G * B and V >= 1 and (step == 1 or V == 1) and (ld >= V or rows <= 1)
     assert out_scores.shape[0] == G and out_beams.shape == out_tokens.shape == out_scores.shape
     assert scores.is_contiguous() and out_scores.is_contiguous() and out_beams.is_contiguous() and out_tokens.is_contiguous()
-    if not beam_select_takes(B, n) or rows > 65535:
-        raise KernelError(f"beam_select: {G} requests of {B} beams, {n} continuations each (at most 65,535 rows, 1,024 beams, "
-                          f"{BEAM_MAX_KEEP} continuations)")
+    if not beam_select_takes(B, n) or rows > 65535 or V > 1 << 30:
+        raise KernelError(f"beam_select: {G} requests of {B} beams, {n} continuations each, of {V} tokens (at most 65,535 rows, 1,024 beams, "
+                          f"{BEAM_MAX_KEEP} continuations, 2^30 tokens)")
     if G == 0:
         return
     key = (rows, V, n, logits.get_device())     # (how rows are cut depends on the device's SMs)
@@ -1244,6 +1244,7 @@ def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, moves) -> None:
     assert _rows_together(k_pool, 1) and _rows_together(v_pool, 1)
     entry = k_pool.stride(0) if E > 1 else P * H * T * D
     assert E == 1 or (v_pool.stride(0) == entry and entry >= P * H * T * D)
+    moves = list(moves)
     sources, firsts, destinations = copy_groups(moves, P)
     positions: dict = {}
     for m in moves:

@@ -221,6 +221,9 @@ def test_page_copies_of_one_entry_and_of_every_other():
     assert torch.equal(k, want_k) and torch.equal(v, want_v)
     ops.copy_pages(k, v, [])
     assert torch.equal(k, want_k)
+    ops.copy_pages(k, v, (m for m in [(5, 4, 64)]))       # any iterable
+    want_k[:, 4], want_v[:, 4] = want_k[:, 5], want_v[:, 5]
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
 
 
 @pytest.mark.parametrize("dtype, shape", [(torch.float32, (149504,)), (torch.float32, (3,)), (torch.float32, (4097,)), (torch.bfloat16, (5, 7)),
