@@ -29,6 +29,7 @@ class PagePool:
         self.n_pages = n_pages
         self._free = list(range(n_pages - 1, -1, -1))  # pop() hands out low ids first
         self._holders = [0] * n_pages
+        self.n_shared = 0                             # pages with more than one holder
 
     @property
     def n_free(self) -> int:
@@ -55,6 +56,8 @@ class PagePool:
             if not (0 <= p < self.n_pages) or self._holders[p] == 0:
                 raise CacheError(f"page {p} is not held and cannot be shared")
             self._holders[p] += 1
+            if self._holders[p] == 2:
+                self.n_shared += 1
 
     def free(self, pages) -> None:
         pages = list(pages)
@@ -64,6 +67,8 @@ class PagePool:
             if self._holders[p] == 0:
                 raise CacheError(f"page {p} freed twice")
             self._holders[p] -= 1
+            if self._holders[p] == 1:
+                self.n_shared -= 1
         self._free.extend(p for p in reversed(pages) if self._holders[p] == 0)
 
 

@@ -470,20 +470,31 @@ class SequenceCache:
         for slot, _ in requests:
             if slot not in self._length:
                 raise CacheError(f"slot {slot} is not live")
-        writers = list(dict.fromkeys(slot for slot, n_new in requests if n_new > 0))
-        for g, n in zip(self.paged_groups, self.pages_needed(requests)):
-            n += g.shared_writes(writers, self._length)
+        lengths = self._length
+        growing = []            # per paged group, the (slot, new length) that need more pages
+        shared = [g for g in self.paged_groups if g.pool.n_shared]
+        writers = list(dict.fromkeys(slot for slot, n_new in requests if n_new > 0)) if shared else []
+        for g in self.paged_groups:
+            more, n = [], 0
+            for slot, n_new in requests:
+                extra = g.pages_needed(slot, lengths[slot] + n_new)
+                if extra > 0:
+                    more.append((slot, lengths[slot] + n_new))
+                    n += extra
+            if g.pool.n_shared:
+                n += g.shared_writes(writers, lengths)
             if n > g.pool.n_free:
                 raise CacheFull(f"cache group {g.index} needs {n} more page(s) of {PAGE_TOKENS} tokens, "
                                 f"{g.pool.n_free} of {g.pool.n_pages} are free")
-        for g in self.paged_groups:
-            moves = g.make_own(writers, self._length)
+            growing.append(more)
+        for g in shared:
+            moves = g.make_own(writers, lengths)
             if moves:
                 self.ownership_changes += 1
                 g.copy(moves)
-        for slot, n_new in requests:
-            for g in self.paged_groups:
-                g.reserve(slot, self._length[slot] + n_new)
+        for g, more in zip(self.paged_groups, growing):
+            for slot, new_length in more:
+                g.reserve(slot, new_length)
 
     def commit(self, slot: int, n_new: int) -> None:
         """The step wrote ``n_new`` tokens: advance the length, let windowed groups drop pages that

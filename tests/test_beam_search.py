@@ -22,10 +22,11 @@ def test_a_shared_page_is_free_after_its_last_holder():
     a, b = pool.alloc(2)
     pool.share([a])
     pool.share([a, b])
-    assert pool.holders(a) == 3 and pool.holders(b) == 2 and pool.n_held == 2
+    assert pool.holders(a) == 3 and pool.holders(b) == 2 and pool.n_held == 2 and pool.n_shared == 2
     pool.free([a, b])
+    assert pool.n_shared == 1
     pool.free([a])
-    assert pool.n_free == 1 and pool.n_held == 2
+    assert pool.n_shared == 0 and pool.n_free == 1 and pool.n_held == 2
     pool.free([b, a])
     assert pool.n_free == 3
     with pytest.raises(CacheError, match="twice"):
