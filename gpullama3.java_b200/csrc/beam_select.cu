@@ -69,6 +69,26 @@ __device__ __forceinline__ u64 beam_key(float x, int token) { return ((u64)risin
 __device__ __forceinline__ float key_logit(u64 key) { return from_rising_bits((unsigned)(key >> 32)); }
 __device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (unsigned)key); }
 
+// Exponentials are taken relative to whole numbers, so that what stands between two sums is a power e^-n, looked up in 64 bits (whose functions take
+// longer than all the rest of a merge); beyond 63 it is below what a sum in 64 bits keeps of the larger one's rounding in 32.
+__constant__ double kPowers[64] = {
+    1.00000000000000000e+00, 3.67879441171442334e-01, 1.35335283236612702e-01, 4.97870683678639445e-02, 1.83156388887341787e-02, 6.73794699908546700e-03,
+    2.47875217666635849e-03, 9.11881965554516244e-04, 3.35462627902511853e-04, 1.23409804086679561e-04, 4.53999297624848542e-05, 1.67017007902456593e-05,
+    6.14421235332820981e-06, 2.26032940698105424e-06, 8.31528719103567877e-07, 3.05902320501825786e-07, 1.12535174719259116e-07, 4.13993771878516683e-08,
+    1.52299797447126292e-08, 5.60279643753726783e-09, 2.06115362243855787e-09, 7.58256042791190660e-10, 2.78946809286892464e-10, 1.02618796317018902e-10,
+    3.77513454427909773e-11, 1.38879438649640209e-11, 5.10908902806332510e-12, 1.87952881653908324e-12, 6.91440010694020302e-13, 2.54366564737692275e-13,
+    9.35762296884017482e-14, 3.44247710846997675e-14, 1.26641655490941755e-14, 4.65888614510339774e-15, 1.71390843154201300e-15, 6.30511676014698922e-16,
+    2.31952283024356963e-16, 8.53304762574406580e-17, 3.13913279204802960e-17, 1.15482241730157861e-17, 4.24835425529158887e-18, 1.56288218933498879e-18,
+    5.74952226429355990e-19, 2.11513103759108046e-19, 7.78113224113379661e-20, 2.86251858054939366e-20, 1.05306173575538117e-20, 3.87399762868718678e-21,
+    1.42516408274093515e-21, 5.24288566336346390e-22, 1.92874984796391782e-22, 7.09547416228470366e-23, 2.61027906966770474e-23, 9.60268005450867556e-24,
+    3.53262857220080711e-24, 1.29958142500750312e-24, 4.78089288388546882e-25, 1.75879220242431161e-25, 6.47023492564545988e-26, 2.38026640869440067e-26,
+    8.75651076269652004e-27, 3.22134028599251593e-27, 1.18506486423398097e-27, 4.35961000006308085e-28,
+};
+__device__ __forceinline__ double brought_to(double sum, float from, float to) {     // from <= to, whole numbers or -inf (a sum of 0, or NaN)
+    const float n = to - from;
+    return n < 64.f ? sum * kPowers[(int)n] : (n >= 64.f && !isnan(sum) ? 0.0 : sum);
+}
+
 struct RowsShared {
     u64 list[kBeamList];                // 36 KB
     int n;
@@ -202,7 +222,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
         if (base == first) {
             // What about the keep-th largest of the threads' maxima reach, at least `keep` logits do, and few more.
             const unsigned key = isnan(mine) ? 0u : rising_bits(mine), top = __reduce_max_sync(0xffffffffu, key);
-            ref = top ? from_rising_bits(top) : -INFINITY;
+            ref = top ? ceilf(from_rising_bits(top)) : -INFINITY;
             unsigned least = 0;
             for (int bit = 31; bit >= 0; --bit) {
                 const unsigned t = least | (1u << bit);
@@ -215,8 +235,9 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
             border = from_rising_bits(max(least, kRisingMinusInf + 1u));     // -inf is no candidate
         }
         if (mine > ref + 16.f) {        // (relative to the maximum of the warp's first logits until that is exceeded by far)
-            if (ref > -INFINITY) total *= (double)expf(ref - mine);
-            ref = mine;
+            const float higher = ceilf(mine);
+            total = ref > -INFINITY ? brought_to(total, ref, higher) : total;
+            ref = higher;
         }
         const float zero = ref == -INFINITY ? 0.f : ref;     // (nothing but -inf so far, or NaN, which has to show)
         float sum[2] = {0.f, 0.f};
@@ -242,7 +263,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
     }
     {
         const float r = warp_max(ref);
-        if (ref < r && ref > -INFINITY) total *= exp((double)ref - (double)r);
+        if (ref < r && ref > -INFINITY) total = brought_to(total, ref, r);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         if (lane == 0) { sh.ref[warp] = r; sh.sum[warp] = total; }
@@ -252,7 +273,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
     if (warp == 0) {
         const float w = lane < kBeamWarps ? sh.ref[lane] : -INFINITY, r = warp_max(w);
         double t = lane < kBeamWarps ? sh.sum[lane] : 0.0;
-        if (w < r && w > -INFINITY) t *= exp((double)w - (double)r);
+        if (w < r && w > -INFINITY) t = brought_to(t, w, r);
 #pragma unroll
         for (int o = kBeamWarps / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
         if (lane == 0) { out.maxima[piece] = r; out.sums[piece] = t; }
@@ -260,17 +281,20 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
     // in order: every candidate's place is the number of those before it
     const int found = sh.n;
     u64* to = out.candidates + piece * keep;
-    for (int i = tid; i < found; i += kBeamThreads) {
-        const u64 key = sh.list[i];
+    for (int i0 = 0; i0 < found; i0 += kBeamThreads / 4) {      // four threads a candidate
+        const int i = i0 + (tid >> 2);
+        const u64 key = i < found ? sh.list[i] : ~0ull;
         int before = 0;
-        for (int k = 0; k < found; ++k) before += sh.list[k] > key ? 1 : 0;
-        if (before < keep) to[before] = key;
+        for (int k = tid & 3; k < found; k += 4) before += sh.list[k] > key ? 1 : 0;
+        before += __shfl_xor_sync(0xffffffffu, before, 1);
+        before += __shfl_xor_sync(0xffffffffu, before, 2);
+        if (i < found && before < keep && (tid & 3) == 0) to[before] = key;
     }
     for (int i = found + tid; i < keep; i += kBeamThreads) to[i] = 0ull;
 }
 
 struct Candidate {
-    double total;
+    u64 total;              // a number that rises with it
     float logit;
     int beam, token;        // token -1: none
 };
@@ -282,30 +306,43 @@ __device__ __forceinline__ bool goes_before(const Candidate& a, const Candidate&
     if (a.logit != b.logit) return a.logit > b.logit;
     return a.token < b.token;
 }
+__device__ __forceinline__ u64 rising_bits(double x) {
+    const u64 b = (u64)__double_as_longlong(x + 0.0);
+    return (b >> 63) ? ~b : b | (1ull << 63);
+}
+__device__ __forceinline__ double double_of(u64 r) { return __longlong_as_double((long long)((r >> 63) ? r & ~(1ull << 63) : ~r)); }
 
 constexpr int kMergeEach = 8, kMergeKeys = kMergeEach * kMergeThreads;
 constexpr int kMergeWarps = kMergeThreads / 32;
 struct MergeShared {
-    u64 keys[kMergeKeys];               // total (rounded down to 32 bits) and number of candidates
-    double total[kMergeList];
+    u64 keys[kMergeKeys];               // rough total and number of candidates
+    u64 total[kMergeList];
     float logit[kMergeList];
     int beam[kMergeList], token[kMergeList];
     int active[kMergeList];             // lists that may hold some of the best
     Candidate warp_best[kMergeWarps];
     int count[2][kMergeWarps];
+    unsigned high[kMergeWarps];
     int n_keys, n_active, n;
+    unsigned largest;                   // of the beams' |base|, its bits
+};
+struct Beam {
+    double exact;       // score - log of the row's sum of exponentials (NaN: the row gives none)
+    float ref;          // what the sum is relative to
+    float base;         // the first, rounded
 };
 
+// 64-bit arithmetic is slow on this chip (a comparison of 80 by 80 totals took 8 us), so candidates are found by rough totals in 32 bits, off by
+// at most half a step of each of their three parts, with a border lowered by more than that; exact totals are made of those that
+// reach it, about as many as are wanted, and are put in order as whole numbers.
 __global__ void __launch_bounds__(kMergeThreads)
 beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int keep, BeamScratch in, float* __restrict__ out_scores,
                   int* __restrict__ out_beams, int* __restrict__ out_tokens) {
     extern __shared__ __align__(16) unsigned char merge_smem[];
     MergeShared& sh = *reinterpret_cast<MergeShared*>(merge_smem);
-    // [beams] what a row's sum is relative to, and the score less the sum's log (NaN: the row gives none): added to a logit in that order, so that
-    // nothing is lost where all of a row is far from 0
-    double2* offset_s = reinterpret_cast<double2*>(merge_smem + sizeof(MergeShared));
+    Beam* beam_s = reinterpret_cast<Beam*>(merge_smem + sizeof(MergeShared));
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) sh.n = sh.n_active = sh.n_keys = 0;
+    if (tid == 0) { sh.n = sh.n_active = sh.n_keys = 0; sh.largest = 0; }
     pdl_launch_dependents();
     pdl_wait();
     const int lists = beams * chunks;       // in the order of beams
@@ -313,91 +350,115 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
     const u64* from = in.candidates + (size_t)g * all;
     // where all candidates fit the threads' registers they are asked for before anything else
     const bool at_once = all <= kMergeKeys;
+    const unsigned chunks_magic = 0xffffffffu / (unsigned)chunks + 1u, keep_magic = 0xffffffffu / (unsigned)keep + 1u;      // 2^32 / d, rounded up
     u64 held[kMergeEach];
     if (at_once) {
 #pragma unroll
         for (int u = 0; u < kMergeEach; ++u) held[u] = tid + u * kMergeThreads < all ? from[tid + u * kMergeThreads] : 0ull;
     }
     for (int b = warp; b < beams; b += kMergeWarps) {
-        const size_t row = (size_t)g * beams + b;
-        const float score = scores[row];
-        float m0 = -INFINITY;
-        double s0 = 0.0;
-        if (lane < chunks) { m0 = in.maxima[row * chunks + lane]; s0 = in.sums[row * chunks + lane]; }     // (what lies there for a row that was not read is not used)
-        double offset = NAN;
-        if (fabsf(score) < INFINITY) {
-            float top = m0;
-            for (int c = lane + 32; c < chunks; c += 32) top = fmaxf(top, in.maxima[row * chunks + c]);
+        const size_t row = ((size_t)g * beams + b) * chunks;
+        const float score = scores[(size_t)g * beams + b];
+        double base = NAN;
+        float top = -INFINITY;
+        if (fabsf(score) < INFINITY) {          // (nothing was left for other rows)
+            for (int c = lane; c < chunks; c += 32) top = fmaxf(top, in.maxima[row + c]);
             top = warp_max(top);
-            double total = m0 > -INFINITY && m0 != top ? s0 * exp((double)m0 - (double)top) : s0;
-            for (int c = lane + 32; c < chunks; c += 32) {
-                const float mc = in.maxima[row * chunks + c];
-                const double s = in.sums[row * chunks + c];
-                total += mc > -INFINITY ? s * exp((double)mc - (double)top) : s;
+            double total = 0.0;
+            for (int c = lane; c < chunks; c += 32) {
+                const float mc = in.maxima[row + c];
+                const double s = in.sums[row + c];
+                total += mc > -INFINITY && mc < top ? brought_to(s, mc, top) : s;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
             // (a NaN sum gives NaN)
-            if (top > -INFINITY && top < INFINITY && total < (double)INFINITY) offset = (double)score - log(total);
-            m0 = top;
+            if (top > -INFINITY && top < INFINITY && total < (double)INFINITY) base = (double)score - log(total);
         }
-        if (lane == 0) offset_s[b] = make_double2((double)m0, offset);
+        if (lane == 0) {
+            beam_s[b] = Beam{base, top, (float)base};
+            if (!isnan(base)) atomicMax(&sh.largest, __float_as_uint(fabsf((float)base)));
+        }
     }
     __syncthreads();
 
-    auto decode = [&](u64 key, int list) {
-        Candidate c{-INFINITY, -INFINITY, 0, -1};
+    auto beam_of = [&](int list) { return chunks == 1 ? list : (int)__umulhi((unsigned)list, chunks_magic); };       // (exact below 2^16)
+    auto list_of = [&](unsigned number) { return at_once ? (keep == 1 ? (int)number : (int)__umulhi(number, keep_magic)) : (int)(number / keep); };
+    auto key_at = [&](int list, int k) { return list < lists && k < keep ? from[(size_t)list * keep + k] : 0ull; };
+    // a candidate's rough total, as a number that rises with it; 0: none
+    auto rough = [&](u64 key, int list) {
+        if (key == 0ull) return 0u;
+        const Beam& b = beam_s[beam_of(list)];
+        const float t = (key_logit(key) - b.ref) + b.base;
+        return isnan(t) ? 0u : rising_bits(t);
+    };
+    auto exact = [&](u64 key, int list) {
+        Candidate c{0ull, -INFINITY, 0, -1};
         if (key == 0ull) return c;
-        c.beam = list / chunks;
-        const double2 offset = offset_s[c.beam];
-        if (isnan(offset.y)) return c;
+        c.beam = beam_of(list);
+        const Beam& b = beam_s[c.beam];
+        if (isnan(b.base)) return c;
         c.token = key_token(key);
         c.logit = key_logit(key);
-        c.total = ((double)c.logit - offset.x) + offset.y;
+        c.total = rising_bits(((double)c.logit - (double)b.ref) + b.exact);
         return c;
     };
-    auto candidate = [&](int list, int k) { return decode(list < lists && k < keep ? from[(size_t)list * keep + k] : 0ull, list); };
-    // a candidate's total rounded down to 32 bits, as a number that rises with it; 0: none
-    auto rounded = [&](const Candidate& c) { return c.token >= 0 ? rising_bits(__double2float_rd(c.total)) : 0u; };
-    // the largest number that `need` of all threads' keys reach (0: there are not as many), or one that few more do
-    auto search = [&](auto count_mine, int need) {
-        unsigned least = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const unsigned t = least | (1u << bit);
+    // what is taken when `least` is what enough rough totals reach: everything that may be exactly as large
+    auto lowered = [&](unsigned least) {
+        const float t = from_rising_bits(least);
+        return max(rising_bits(t - 4.8e-7f * (fabsf(t) + __uint_as_float(sh.largest))), 1u);      // (8 half steps of either)
+    };
+    // The largest number that `need` of all threads' keys reach (0: there are not as many), or one that few more do; `mine`: the thread's largest.  What
+    // lies above the largest of all, and the bits that numbers between it and the least of the warps' largest have in common, are not searched where
+    // those are enough already.
+    auto search = [&](auto count_mine, unsigned mine, int need) {
+        mine = __reduce_max_sync(0xffffffffu, mine);
+        if (lane == 0) sh.high[warp] = mine;
+        __syncthreads();
+        const unsigned w = lane < kMergeWarps ? sh.high[lane] : 0u, high = __reduce_max_sync(0xffffffffu, w);
+        auto reaching = [&](unsigned t, int set) {
             int n = __reduce_add_sync(0xffffffffu, count_mine(t));
-            if (lane == 0) sh.count[bit & 1][warp] = n;     // (two sets of counts in turn: one barrier a count)
+            if (lane == 0) sh.count[set][warp] = n;         // (two sets of counts in turn: one barrier a count)
             __syncthreads();
-            n = __reduce_add_sync(0xffffffffu, lane < kMergeWarps ? sh.count[bit & 1][lane] : 0);
+            return (int)__reduce_add_sync(0xffffffffu, lane < kMergeWarps ? sh.count[set][lane] : 0);
+        };
+        // numbers that differ from the largest in their last 24 bits only: totals within a factor of four or so
+        unsigned least = high & 0xff000000u;
+        int bit = 23;
+        if (reaching(least, 0) < need) { least = 0; bit = 31; }
+        for (; bit >= 0; --bit) {
+            const unsigned t = least | (1u << bit);
+            const int n = t <= high ? reaching(t, bit & 1 ^ 1) : 0;
             if (n >= need) {
                 least = t;
                 if (n <= need + need / 4) break;
             }
         }
-        return max(least, 1u);
+        return least ? lowered(least) : 1u;
     };
     unsigned least = 1;
     bool listed = true;         // what may be among the best has gone to the list
-    u64 mine[kMergeEach];       // total and number
+    u64 mine[kMergeEach];       // rough total and number
     if (at_once) {
 #pragma unroll
         for (int u = 0; u < kMergeEach; ++u) {
             const int i = tid + u * kMergeThreads;
-            mine[u] = ((u64)rounded(decode(held[u], i / keep)) << 32) | (unsigned)i;
+            mine[u] = ((u64)rough(held[u], list_of(i)) << 32) | (unsigned)i;
         }
     } else {
         // A number that at least `keep` candidates reach and not many more: where there are lists enough, one that `keep` of the threads'
         // best heads reach; where there are few, one that so many of their (depth + 1)-th best reach that it comes to as much.
         bool head = false;
-        for (int l = tid; l < lists; l += kMergeThreads) head = head || candidate(l, 0).token >= 0;
+        for (int l = tid; l < lists; l += kMergeThreads) head = head || rough(key_at(l, 0), l) != 0u;
         const int n_heads = __syncthreads_count(head);
         const int depth = n_heads >= keep || n_heads == 0 ? 0 : (2 * keep + n_heads - 1) / n_heads - 1;
         unsigned key = 0;
-        for (int l = tid; l < lists; l += kMergeThreads) key = max(key, rounded(candidate(l, depth)));
-        least = search([&](unsigned t) { return key >= t ? 1 : 0; }, (keep + depth) / (depth + 1));
+        for (int l = tid; l < lists; l += kMergeThreads) key = max(key, rough(key_at(l, depth), l));
+        least = search([&](unsigned t) { return key >= t ? 1 : 0; }, key, (keep + depth) / (depth + 1));
         __syncthreads();
         // the lists with a candidate that reaches it, a thread each; then of those, a warp each, all that reach it
         for (int l = tid; l < lists; l += kMergeThreads) {
-            if (rounded(candidate(l, 0)) >= least) {
+            if (rough(key_at(l, 0), l) >= least) {
                 const int i = atomicAdd(&sh.n_active, 1);
                 if (i < kMergeList) sh.active[i] = l;
             }
@@ -406,7 +467,7 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         const int n_active = sh.n_active;
         for (int a = warp; a < min(n_active, kMergeList); a += kMergeWarps) {
             for (int k0 = 0; k0 < keep; k0 += 32) {
-                const unsigned b = rounded(candidate(sh.active[a], k0 + lane));
+                const unsigned b = rough(key_at(sh.active[a], k0 + lane), sh.active[a]);
                 const bool in = b >= least;
                 if (in) {
                     const int i = atomicAdd(&sh.n_keys, 1);
@@ -421,17 +482,20 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         for (int u = 0; u < kMergeEach; ++u) mine[u] = tid + u * kMergeThreads < min(sh.n_keys, kMergeKeys) ? sh.keys[tid + u * kMergeThreads] : 0ull;
     }
     if (listed) {
+        unsigned best = 0;
+#pragma unroll
+        for (int u = 0; u < kMergeEach; ++u) best = max(best, (unsigned)(mine[u] >> 32));
         least = search([&](unsigned t) {
             int n = 0;
 #pragma unroll
             for (int u = 0; u < kMergeEach; ++u) n += (unsigned)(mine[u] >> 32) >= t ? 1 : 0;
             return n;
-        }, keep);
+        }, best, keep);
 #pragma unroll
         for (int u = 0; u < kMergeEach; ++u) {
             if ((unsigned)(mine[u] >> 32) >= least) {
                 const unsigned number = (unsigned)mine[u];
-                const Candidate c = at_once ? decode(held[u], number / keep) : candidate(number / keep, number % keep);
+                const Candidate c = exact(at_once ? held[u] : from[number], list_of(number));
                 const int i = atomicAdd(&sh.n, 1);
                 if (i < kMergeList) { sh.total[i] = c.total; sh.logit[i] = c.logit; sh.beam[i] = c.beam; sh.token[i] = c.token; }
             }
@@ -441,16 +505,19 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
     const size_t to = (size_t)g * keep;
     const int found = listed ? sh.n : kMergeList + 1;
     if (found <= kMergeList) {
-        for (int i = tid; i < found; i += kMergeThreads) {
-            const Candidate c{sh.total[i], sh.logit[i], sh.beam[i], sh.token[i]};
+        for (int i0 = 0; i0 < found; i0 += kMergeThreads / 4) {         // four threads a candidate
+            const int i = i0 + (tid >> 2), at = min(i, found - 1);
+            const Candidate c{sh.total[at], sh.logit[at], sh.beam[at], sh.token[at]};
             int before = 0;
-            for (int k = 0; k < found; ++k) {
-                const double o = sh.total[k];
-                if (o > c.total) ++before;
-                else if (o == c.total) before += goes_before(Candidate{o, sh.logit[k], sh.beam[k], sh.token[k]}, c) ? 1 : 0;
+            for (int k = tid & 3; k < found; k += 4) {
+                const u64 o = sh.total[k];
+                before += o > c.total ? 1 : 0;
+                if (o == c.total && k != at) before += goes_before(Candidate{o, sh.logit[k], sh.beam[k], sh.token[k]}, c) ? 1 : 0;
             }
-            if (before < keep) {
-                out_scores[to + before] = (float)c.total;
+            before += __shfl_xor_sync(0xffffffffu, before, 1);
+            before += __shfl_xor_sync(0xffffffffu, before, 2);
+            if (i < found && before < keep && (tid & 3) == 0) {
+                out_scores[to + before] = (float)double_of(c.total);
                 out_beams[to + before] = c.beam;
                 out_tokens[to + before] = c.token;
             }
@@ -464,12 +531,12 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
     }
     // More than the list holds reach the border (many equal totals): the best head of all lists, `keep` times.  What a thread has
     // taken from its lists is found again by the order: it hands out what comes behind the last one taken from all.
-    Candidate last{INFINITY, INFINITY, -1, INT_MAX};
+    Candidate last{~0ull, INFINITY, -1, INT_MAX};
     for (int r = 0; r < keep; ++r) {
-        Candidate best{-INFINITY, -INFINITY, 0, -1};
+        Candidate best{0ull, -INFINITY, 0, -1};
         for (int l = tid; l < lists; l += kMergeThreads) {
             for (int k = 0; k < keep; ++k) {
-                const Candidate c = candidate(l, k);
+                const Candidate c = exact(key_at(l, k), l);
                 if (c.token < 0) break;
                 if (r > 0 && !goes_before(last, c)) continue;
                 if (goes_before(c, best)) best = c;
@@ -492,7 +559,7 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         __syncthreads();
         last = best;
         if (tid == 0) {
-            out_scores[to + r] = best.token >= 0 ? (float)best.total : -INFINITY;
+            out_scores[to + r] = best.token >= 0 ? (float)double_of(best.total) : -INFINITY;
             out_beams[to + r] = best.token >= 0 ? best.beam : -1;
             out_tokens[to + r] = best.token;
         }
@@ -536,12 +603,12 @@ extern "C" int b200_beam_select(const float* logits, long long ld, const float* 
     if (scratch_bytes < b200_beam_select_scratch_bytes((int)rows, vocab, keep)) return 10003;
     const BeamScratch s = beam_scratch(scratch, rows * chunks, keep);
     const int vec = ((uintptr_t)logits & 15) == 0 && (ld & 3) == 0;
-    const size_t merge_bytes = sizeof(MergeShared) + sizeof(double2) * beams;
+    const size_t merge_bytes = sizeof(MergeShared) + sizeof(Beam) * beams;
     static bool configured[64] = {};
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
     if (!configured[device]) {
-        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(MergeShared) + sizeof(double2) * 1024));
+        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(MergeShared) + sizeof(Beam) * 1024));
         if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
         configured[device] = true;
     }
