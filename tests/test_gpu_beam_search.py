@@ -201,3 +201,47 @@ def test_command_line_searches(session_tmp):
     assert r.returncode == 0, r.stderr
     assert [[int(t) for t in line.split()] for line in r.stdout.strip().splitlines()] == want
     assert "achieved tok/s" in r.stderr
+
+
+@pytest.mark.parametrize("family, name", [("llama", "B"), ("guduzen", "A"), ("gatuzen", "A")])
+def test_forked_sequences_go_on_by_ordinary_steps(session_tmp, family, name):
+    """Forks of one sequence, continued by single tokens (recorded steps), by chunks and by chunks of unequal length in one step, give
+    the logits of sequences that were told the same from their beginning."""
+    from conftest import assert_close_logits
+    from gpullama3.java_b200.engine.api import Engine, SequenceInput
+
+    if family == "llama":
+        d = make_model_dir(session_tmp, TINY[name][0], seed=21, norm_std=0.1, scale=SCALE)
+    else:
+        helpers = importlib.import_module(f"{family}_helpers")
+        d = getattr(helpers, f"make_{family}_dir")(session_tmp, helpers.CONFIGS[name], seed=11)
+    engine = Engine.from_folder(d, dtype="float32", max_tokens=64 * 40, max_batch=8)
+    vocab = engine.config.vocab_size
+    prompt, *more = random_prompts(vocab, [70, 5, 64, 1, 130], seed=4)
+    cache, step = engine.cache, engine.step
+    first = cache.acquire()
+    step([SequenceInput(first, prompt, [])])
+    slots = [first] + cache.fork([first] * (len(more) - 1))
+    told = [list(prompt) for _ in more]
+    for turn in range(3):                             # single tokens of all, twice the recorded step
+        tokens = random_prompts(vocab, [1] * len(more), seed=50 + turn)
+        got = step([SequenceInput(s, t, [0]) for s, t in zip(slots, tokens)])
+        for i, t in enumerate(tokens):
+            told[i] += t
+    chunks = step([SequenceInput(s, t, [len(t) - 1]) for s, t in zip(slots, more)])
+    again = cache.fork([slots[3]])[0]                 # a fork of a fork, behind a page border or not
+    tail = random_prompts(vocab, [2], seed=9)[0]
+    last = step([SequenceInput(again, tail, [0, 1])])
+    for rows, histories in ((got, told), (chunks, [a + b for a, b in zip(told, more)])):
+        for i, history in enumerate(histories):
+            s = cache.acquire()
+            want = step([SequenceInput(s, history, [len(history) - 1])])
+            cache.release(s)
+            assert_close_logits(rows[i:i + 1], want, torch.float32, f"sequence {i}")
+    s = cache.acquire()
+    history = told[3] + more[3] + tail
+    want = step([SequenceInput(s, history, [len(history) - 2, len(history) - 1])])
+    assert_close_logits(last, want, torch.float32, "fork of a fork")
+    cache.check_invariants()
+    for s in cache.live_slots():
+        cache.release(s)
