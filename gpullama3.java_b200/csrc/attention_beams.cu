@@ -54,8 +54,14 @@ __device__ __forceinline__ int first_key(int kv_len, int window) { return window
 
 // Segments: part p of n_parts = n_groups * n_sub (n_sub parts of up to sub_beams sequences to a group) has its shared pages as segment
 // p * (sub_beams + 1), its sequences' own as the next ones.
-__device__ __forceinline__ int part_first_row(const BeamAttnArgs& a, int p) { return (p / a.n_sub) * a.beams + (p % a.n_sub) * a.sub_beams; }
-__device__ __forceinline__ int part_rows(const BeamAttnArgs& a, int p) { return min(a.sub_beams, a.beams - (p % a.n_sub) * a.sub_beams); }
+__device__ __forceinline__ int part_first_row(const BeamAttnArgs& a, int p) {
+    if (a.n_sub == 1) return p * a.beams;
+    const int g = p / a.n_sub;
+    return g * a.beams + (p - g * a.n_sub) * a.sub_beams;
+}
+__device__ __forceinline__ int part_rows(const BeamAttnArgs& a, int p) {
+    return a.n_sub == 1 ? a.beams : min(a.sub_beams, a.beams - (p % a.n_sub) * a.sub_beams);
+}
 
 __device__ __forceinline__ int part_of_segment(const BeamAttnArgs& a, int s) { return (int)__umulhi((unsigned)s, a.per_magic); }   // (s below 2^16)
 
@@ -154,21 +160,26 @@ __global__ void __launch_bounds__(256) attention_beams_plan_kernel(const __grid_
     for (int i = threadIdx.x; i <= a.n_segments; i += 256) reinterpret_cast<int4*>(a.plan)[i] = reinterpret_cast<const int4*>(seg)[i];
 }
 
-// the last of the segments that begin at or before `x` on the line (by_pages: before whose end page number x lies, and which is not empty)
-template <bool BY_PAGES>
-__device__ __forceinline__ int segment_at(const BeamAttnArgs& a, const Segment* seg, int x) {
+// the segment of page number u: the last one that begins at or before it, which is not an empty one
+__device__ __forceinline__ int segment_of(const BeamAttnArgs& a, const Segment* seg, int u) {
     int lo = 0, hi = a.n_segments - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if ((BY_PAGES ? seg[mid].pages : seg[mid].at) <= x) lo = mid; else hi = mid - 1;
+        if (seg[mid].pages <= u) lo = mid; else hi = mid - 1;
     }
     return lo;
 }
-// the number of pages that begin before place x of the line
-__device__ __forceinline__ int pages_before(const BeamAttnArgs& a, const Segment* seg, int x) {
-    if (x >= seg[a.n_segments].at) return seg[a.n_segments].pages;
-    const int s = segment_at<false>(a, seg, x);
-    return seg[s].pages + min(max(x - seg[s].at - kSegmentCost, 0), seg[s + 1].pages - seg[s].pages);
+// the numbers of the pages that begin before places x and y of the line
+__device__ __forceinline__ int2 pages_before(const BeamAttnArgs& a, const Segment* seg, int x, int y) {
+    int lx = 0, hx = a.n_segments - 1, ly = 0, hy = hx;
+    while (lx < hx || ly < hy) {
+        const int mx = (lx + hx + 1) >> 1, my = (ly + hy + 1) >> 1;
+        const int ax = seg[mx].at, ay = seg[my].at;
+        if (lx < hx) { if (ax <= x) lx = mx; else hx = mx - 1; }
+        if (ly < hy) { if (ay <= y) ly = my; else hy = my - 1; }
+    }
+    auto before = [&](int s, int z) { return seg[s].pages + min(max(z - seg[s].at - kSegmentCost, 0), seg[s + 1].pages - seg[s].pages); };
+    return make_int2(before(lx, x), before(ly, y));
 }
 
 // A page of the work: where it lies, whose it is, its first position, and how many of its keys there are.
@@ -177,7 +188,7 @@ struct Unit {
 };
 __device__ __forceinline__ Unit unit_of(const BeamAttnArgs& a, const Segment* seg, const int* lens, int u) {
     Unit x;
-    x.segment = segment_at<true>(a, seg, u);
+    x.segment = segment_of(a, seg, u);
     const Segment s = seg[x.segment];
     const int index = s.lo + u - s.pages;
     x.page = a.page_table[(size_t)s.row * a.table_stride + index];
@@ -391,7 +402,8 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
     pdl_launch_dependents();
     take_plan<kBaThreads>(a, seg, lens, tmp);
     const int per = stretch_of(seg[a.n_segments].at, gridDim.x);
-    const int u0 = pages_before(a, seg, blockIdx.x * per), u1 = pages_before(a, seg, (blockIdx.x + 1) * per);
+    const int2 mine = pages_before(a, seg, blockIdx.x * per, (blockIdx.x + 1) * per);
+    const int u0 = mine.x, u1 = mine.y;
     if (u0 >= u1) return;
 
     const size_t page_elements = (size_t)a.n_kv_heads * kPageTokens * D, head_off = (size_t)kvh * kPageTokens * D;
@@ -601,7 +613,8 @@ __global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const _
     pdl_launch_dependents();
     take_plan<kBfThreads>(a, seg, lens, tmp);
     const int per = stretch_of(seg[a.n_segments].at, gridDim.x);
-    const int u0 = pages_before(a, seg, blockIdx.x * per), u1 = pages_before(a, seg, (blockIdx.x + 1) * per);
+    const int2 mine = pages_before(a, seg, blockIdx.x * per, (blockIdx.x + 1) * per);
+    const int u0 = mine.x, u1 = mine.y;
     if (u0 >= u1) return;
 
     const size_t page_elements = (size_t)a.n_kv_heads * kPageTokens * D, head_off = (size_t)kvh * kPageTokens * D;
@@ -764,15 +777,21 @@ __global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_
     pdl_launch_dependents();
     if (!a.given) pdl_wait();       // (a given plan was complete before the kernel ahead of this one began its work)
     const Segment* seg = reinterpret_cast<const Segment*>(a.plan);
-    const int line = seg[a.n_segments].at, per = stretch_of(line, n_ctas);
     int c0 = 0, n0 = 0, c1 = 0, n1 = 0;     // the first CTA with pages of the shared segment and their number; the same of its own
     if (mine) {
-        const int s0 = seg[shared].pages, s1 = seg[shared + 1].pages, o0 = seg[own].pages, o1 = seg[own + 1].pages;
-        const int sa = seg[shared].at + kSegmentCost, oa = seg[own].at + kSegmentCost;
-        c0 = sa / per;
-        n0 = s0 < s1 ? (sa + s1 - s0 - 1) / per - c0 + 1 : 0;
-        c1 = oa / per;
-        n1 = o0 < o1 ? (oa + o1 - o0 - 1) / per - c1 + 1 : 0;
+        const int2* of = reinterpret_cast<const int2*>(seg);        // (pages, at) of each
+        const int2 s0 = of[2 * shared], s1 = of[2 * shared + 2], o0 = of[2 * own], o1 = of[2 * own + 2], end = of[2 * a.n_segments];
+        const unsigned per = (unsigned)stretch_of(end.y, n_ctas), magic = per > 1 ? 0xffffffffu / per + 1u : 0u;
+        auto cta_of = [&](int x) {              // x / per
+            if (magic == 0u) return x;
+            const unsigned q = __umulhi((unsigned)x, magic);
+            return (int)((unsigned long long)q * per > (unsigned)x ? q - 1u : q);
+        };
+        const int sa = s0.y + kSegmentCost, oa = o0.y + kSegmentCost, sn = s1.x - s0.x, on = o1.x - o0.x;
+        c0 = cta_of(sa);
+        n0 = sn > 0 ? cta_of(sa + sn - 1) - c0 + 1 : 0;
+        c1 = cta_of(oa);
+        n1 = on > 0 ? cta_of(oa + on - 1) - c1 + 1 : 0;
     }
     if (a.given) pdl_wait();
     if (!mine) return;

@@ -26,7 +26,7 @@ constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamEach = 16;                           // logits of a thread at a time
 constexpr int kBeamTile = kBeamThreads * kBeamEach;
 constexpr int kBeamMaxKeep = 256;
-constexpr int kBeamLimit = 2 * kBeamMaxKeep + 64;       // most candidates of a list that is not cut down
+constexpr int kBeamLimit = kBeamMaxKeep + kBeamMaxKeep / 2 + 32;      // most candidates of a list that is not cut down
 constexpr int kBeamList = kBeamLimit + kBeamTile;       // most that it holds
 constexpr int kMergeThreads = 512;
 constexpr int kMergeList = 1024;
@@ -205,7 +205,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
             for (int e = 0; e < kBeamEach; ++e) x[e] = place(e) < n ? __ldg(x0 + place(e)) : -INFINITY;
         }
     };
-    const int limit = max(128, 2 * keep + 64);
+    const int limit = max(128, keep + keep / 2 + 32);
     float border = 0.f;         // what candidates reach
     float ref = -INFINITY;      // the thread's exponentials are relative to it
     double total = 0.0;
