@@ -7,8 +7,8 @@
 // tile: at 8 beams of 32 heads on 8 that is 32 rows, and an eighth of the bytes that as many separate sequences read.
 //
 // The work is cut by pages.  The pages of one segment belong together: the shared pages of a group, then the pages that each
-// of its sequences has for itself, group after group.  All segments in this order make one line, on which a page is 1 long and a segment with
-// pages kSegmentCost longer (what it costs to begin and leave one); of every kv head each of gridDim.x CTAs takes the pages of an equal
+// of its sequences has for itself, group after group.  All segments in this order make one line, on which a page is 1 long (in float32, where the tensor
+// cores bound it, a shared one 2 or 4 with more than 16 or 32 rows) and a segment with pages kSegmentCost longer (what it costs to begin and leave one); of every kv head each of gridDim.x CTAs takes the pages of an equal
 // stretch, whatever they belong to, so groups of unequal length share the GPU evenly.  The line is laid out by each CTA for itself, or once for all
 // layers of a step by attention_beams_plan.
 // A CTA keeps the running maximum m, sum l and output o of a segment's rows in registers and leaves them, unnormalised, in
@@ -20,6 +20,13 @@
 // value into the page as it lies in shared memory and into the cache.  The page that holds the new position is always a sequence's own.
 //
 // Groups of more than 64 rows to a kv head are cut into equal groups of whole beams, each of which reads the shared pages.
+//
+// Bound by HBM in bytes: every key and value that some row reads, once.  Measured (both kernels, no plan given): 4 groups of 4 beams, 32 heads
+// on 8 of 128, at 2,200 to 16,200 positions, 155 MB in 34.4 us, 5.5 TB/s while the pages stream; 8 groups of 8 beams, 32 heads on 8 of 64, at about
+// 4,100 positions, 76 MB in 28.0 us: 2 us for the line, 1.5 until the first page is there, 17 of pages, 4.5 for the join and the rest for starts
+// and ends; one group of 4 at 920 positions 8.6 us, of which the pages need 0.3.  float32 is bound by the tensor cores (six products for one, 57% of
+// their rate while pages stream): 8 groups of 8 beams, 32 heads on 8 of 64, at about 3,900 positions, 144 MB in 72 us (178 us on
+// multiply-adds, bound by reading queries and probabilities from shared memory).
 #include "common.cuh"
 
 namespace b200 {
@@ -48,6 +55,7 @@ struct BeamAttnArgs {
     unsigned per_magic;                 // 2^32 / (sub_beams + 1), rounded up
     long long q_row_stride;
     int table_stride, n_seqs, n_groups, beams, sub_beams, n_sub, n_parts, n_segments, n_heads, n_kv_heads, window;
+    int length;                         // of a shared page on the line of a plan that is made here, as a power of two
 };
 
 __device__ __forceinline__ int first_key(int kv_len, int window) { return window > 0 ? max(0, kv_len - window) : 0; }
@@ -72,11 +80,16 @@ struct Segment {
     int lo;             // its first page's place in the page table
     int row;            // the sequence whose row of the table that is
 };
-// In shared memory: [n_segments + 1] of these, the last one's `pages` and `at` the ends; then the sequences' lengths (as far as they are
+// In shared memory: [n_segments + 1] of these, the last one's `pages` and `at` the ends, its `row` the length of a shared page (2 to that power); then the sequences' lengths (as far as they are
 // needed) and the parts' shared pages.
 static int plan_ints(const BeamAttnArgs& a) { return 4 * (a.n_segments + 1) + a.n_seqs + 2 * a.n_parts; }
-// the length of a CTA's stretch
-__device__ __forceinline__ int stretch_of(int line, int ctas) { return max(1, (line + ctas - 1) / ctas); }
+// the length of a segment's pages as a power of two, `shared` being that of the shared ones
+__device__ __forceinline__ int page_length(const BeamAttnArgs& a, int s, int shared) {
+    return shared == 0 || part_of_segment(a, s) * (a.sub_beams + 1) != s ? 0 : shared;
+}
+// the length of a CTA's stretch, `end` being the plan's last entry: no shorter than a page, so that every CTA between the first and the last one with
+// pages of a segment has some
+__device__ __forceinline__ int stretch_of(const Segment& end, int ctas) { return max(1 << end.row, (end.at + ctas - 1) / ctas); }
 
 // Lays the line out.  By all threads of a CTA.  `tmp`: two ints for each warp.
 template <int THREADS>
@@ -113,7 +126,7 @@ __device__ __forceinline__ void make_plan(const BeamAttnArgs& a, Segment* seg, i
         }
         seg[s] = Segment{hi - lo, 0, lo, row};
         pages += hi - lo;
-        line += hi > lo ? hi - lo + kSegmentCost : 0;
+        line += hi > lo ? ((hi - lo) << page_length(a, s, a.length)) + kSegmentCost : 0;
     }
     int pages_to = pages, line_to = line;
 #pragma unroll
@@ -130,9 +143,9 @@ __device__ __forceinline__ void make_plan(const BeamAttnArgs& a, Segment* seg, i
         seg[s].pages = pages_before;
         seg[s].at = line_before;
         pages_before += n;
-        line_before += n > 0 ? n + kSegmentCost : 0;
+        line_before += n > 0 ? (n << page_length(a, s, a.length)) + kSegmentCost : 0;
     }
-    if (tid == THREADS - 1) seg[a.n_segments] = Segment{pages_before, line_before, 0, 0};
+    if (tid == THREADS - 1) seg[a.n_segments] = Segment{pages_before, line_before, 0, a.length};
     __syncthreads();
 }
 
@@ -178,7 +191,11 @@ __device__ __forceinline__ int2 pages_before(const BeamAttnArgs& a, const Segmen
         if (lx < hx) { if (ax <= x) lx = mx; else hx = mx - 1; }
         if (ly < hy) { if (ay <= y) ly = my; else hy = my - 1; }
     }
-    auto before = [&](int s, int z) { return seg[s].pages + min(max(z - seg[s].at - kSegmentCost, 0), seg[s + 1].pages - seg[s].pages); };
+    const int length = seg[a.n_segments].row;
+    auto before = [&](int s, int z) {
+        const int power = page_length(a, s, length);
+        return seg[s].pages + min((max(z - seg[s].at - kSegmentCost, 0) + (1 << power) - 1) >> power, seg[s + 1].pages - seg[s].pages);
+    };
     return make_int2(before(lx, x), before(ly, y));
 }
 
@@ -215,6 +232,12 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same without what was in d
+__device__ __forceinline__ void mma_bf16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -225,22 +248,35 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// bfloat16, on mma.sync.  A warp owns a tile of 16 rows and, where there are fewer than four tiles, a part of each page's keys.  Rows of shared
-// memory are such that the eight rows of an ldmatrix block meet no bank twice: 128 or 256 bytes with their 16-byte pieces exchanged
-// by the row's last three bits, others with 16 bytes between them.
+// Both types on mma.sync.  A warp owns a tile of 16 rows and, where there are fewer than four tiles, a part of each page's keys.  Rows of shared memory
+// are such that what lanes read together meets no bank twice: bfloat16, eight rows of an ldmatrix block in rows of 128 or 256 bytes with
+// their 16-byte pieces exchanged by the row's last three bits, others with 16 bytes between them; float32, the halves of 128 bytes exchanged in
+// every other row, of which two are read at a time.
+template <typename E, int D>
+struct BeamTile;
 template <int D>
-struct BeamTile {
+struct BeamTile<__nv_bfloat16, D> {
     static constexpr bool kExchange = D % 64 == 0;
-    static constexpr int kPitchK = kExchange ? 2 * D : 2 * D + 16, kPitchV = 2 * kPageTokens;       // bytes
-    static constexpr int kStage = kPageTokens * kPitchK + D * kPitchV;
+    static constexpr int kPitchK = kExchange ? 2 * D : 2 * D + 16, kPitchV = 2 * kPageTokens, kPitchQ = kPitchK;       // bytes
+    static constexpr int kStage = kPageTokens * kPitchK + D * kPitchV, kPeriod = 8;
+    // As many stages as leave room for three CTAs an SM with heads of up to 64, two with wider ones.
+    static constexpr int kResident = D <= 64 ? 3 : 2, kMore = D <= 64 ? 4 : 3;
     static __device__ __forceinline__ uint32_t k_piece(int row, int c) { return row * kPitchK + ((kExchange ? c ^ (row & 7) : c) << 4); }
     static __device__ __forceinline__ uint32_t v_piece(int row, int c) { return row * kPitchV + ((c ^ (row & 7)) << 4); }
+};
+template <int D>
+struct BeamTile<float, D> {
+    static constexpr int kPitchK = 4 * D, kPitchV = 4 * kPageTokens, kPlaneQ = 2 * D + 16, kPitchQ = 3 * kPlaneQ;       // (queries: three parts, see below)
+    static constexpr int kStage = kPageTokens * kPitchK + D * kPitchV, kPeriod = 2;
+    static constexpr int kResident = D <= 64 ? 2 : 1, kMore = 3;
+    static __device__ __forceinline__ uint32_t k_piece(int row, int c) { return row * kPitchK + ((c ^ ((row & 1) << 2)) << 4); }
+    static __device__ __forceinline__ uint32_t v_piece(int row, int c) { return row * kPitchV + ((c ^ ((row & 1) << 2)) << 4); }
 };
 
 template <int D>
 struct RowState {
     float o[D / 8][4];
-    float m[2], l[4];               // of rows g and g + 8; l twice each
+    float m[2], l[4];               // of rows g and g + 8; l twice each (float32: a lane's share in the first)
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
@@ -259,7 +295,7 @@ template <int D, int NK>
 __device__ __forceinline__ void attend_keys(RowState<D>& st, const uint32_t (&qa)[D / 16][4], uint32_t k_base, uint32_t v_base, int first, int lane,
                                             float scale_log2, bool masked, int position, const int (&row_lo)[2], int row_end) {
     constexpr int NT = NK / 8;
-    using T = BeamTile<D>;
+    using T = BeamTile<__nv_bfloat16, D>;
     float s[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -336,8 +372,107 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const uint32_t (&qa
     }
 }
 
-// Joins the parts that the warps of a tile hold and stores the tile's first `rows` rows at `to_o` and `to_ml`.  All warps of the CTA call it.
+// float32: x = h + m + l, three bfloat16 numbers of 8 bits each (what is left is below 2^-26 of x); a product is h h + (h m + m h) + (m m + h l + l h),
+// six on the tensor cores with an error below that of one product's rounding.  The three magnitudes are added separately, and the output of 16
+// keys before it joins the row's, in 32 bits: a tensor core's own sum drops bits instead of rounding them.
+struct Parts {
+    uint32_t h, m, l;
+};
+__device__ __forceinline__ Parts parts_of(float x, float y) {
+    Parts p;
+    p.h = pack2(x, y);
+    x -= __uint_as_float(p.h << 16);
+    y -= __uint_as_float(p.h & 0xffff0000u);
+    p.m = pack2(x, y);
+    x -= __uint_as_float(p.m << 16);
+    y -= __uint_as_float(p.m & 0xffff0000u);
+    p.l = pack2(x, y);
+    return p;
+}
+struct Sums {
+    float s[3][4];
+    // a: the parts of 16 rows by 16, [part][register]; b0, b1: the parts of two numbers each of this lane's column.  first: nothing has been added yet.
+    __device__ __forceinline__ void add(bool first, const uint32_t (&a)[3][4], const Parts& b0, const Parts& b1) {
+        if (first) {
+            mma_bf16_zero(s[2], a[1], b0.m, b1.m);
+            mma_bf16_zero(s[1], a[0], b0.m, b1.m);
+            mma_bf16_zero(s[0], a[0], b0.h, b1.h);
+        } else {
+            mma_bf16(s[2], a[1], b0.m, b1.m);
+            mma_bf16(s[1], a[0], b0.m, b1.m);
+            mma_bf16(s[0], a[0], b0.h, b1.h);
+        }
+        mma_bf16(s[2], a[0], b0.l, b1.l);
+        mma_bf16(s[1], a[1], b0.h, b1.h);
+        mma_bf16(s[2], a[2], b0.h, b1.h);
+    }
+    __device__ __forceinline__ float total(int c) const { return s[0][c] + (s[1][c] + s[2][c]); }
+};
+
+// 16 keys of a page from its key `first` on.  Dimensions and keys are paired with the matrix instructions' places so that a lane's four numbers of a
+// row are one access: place 2 t + e of sixteen is number 4 t + e, place 8 + 2 t + e number 4 t + 2 + e.  q_row: the lane's row of queries.
 template <int D>
+__device__ __forceinline__ void attend_keys_f32(RowState<D>& st, uint32_t q_row, const unsigned char* k_page, const unsigned char* v_page, int first, int lane,
+                                                float scale, bool masked, int position, const int (&row_lo)[2], int row_end) {
+    using T = BeamTile<float, D>;
+    const int n = lane >> 2, t = lane & 3;
+    Sums sums[2];
+    const int key0 = first + 4 * (n >> 1) + (n & 1);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t qa[3][4];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) ldmatrix4(qa[p], q_row + p * T::kPlaneQ + (ks * 2 + (lane >> 4)) * 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4 k = *reinterpret_cast<const float4*>(k_page + T::k_piece(key0 + 2 * i, ks * 4 + t));
+            sums[i].add(ks == 0, qa, parts_of(k.x, k.y), parts_of(k.z, k.w));
+        }
+    }
+    float s[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            s[i][c] = sums[i].total(c) * scale;
+            const int key = position + first + 4 * t + 2 * i + (c & 1);
+            if (masked && (key < row_lo[c >> 1] || key >= row_end)) s[i][c] = -INFINITY;
+        }
+    float keep[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m = fmaxf(st.m[h], top), base = m == -INFINITY ? 0.f : m;       // (a row that has seen nothing yet: its probabilities are 0)
+        keep[h] = expf(st.m[h] - base);
+        st.m[h] = m;
+        st.l[2 * h] *= keep[h];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[i][2 * h + e] = expf(s[i][2 * h + e] - base);
+                st.l[2 * h] += s[i][2 * h + e];
+            }
+    }
+    const Parts p0 = parts_of(s[0][0], s[0][1]), p1 = parts_of(s[0][2], s[0][3]), p2 = parts_of(s[1][0], s[1][1]), p3 = parts_of(s[1][2], s[1][3]);
+    const uint32_t pa[3][4] = {{p0.h, p1.h, p2.h, p3.h}, {p0.m, p1.m, p2.m, p3.m}, {p0.l, p1.l, p2.l, p3.l}};
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+        const float4 v = *reinterpret_cast<const float4*>(v_page + T::v_piece(8 * j + n, (first >> 2) + t));
+        Sums o;
+        o.add(true, pa, parts_of(v.x, v.y), parts_of(v.z, v.w));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) st.o[j][c] = st.o[j][c] * keep[c >> 1] + o.total(c);
+    }
+}
+
+// What a difference of maxima comes to: they are in units of log 2 where the scores were, in bfloat16.
+template <typename E> __device__ __forceinline__ float weight(float x) { return sizeof(E) == 2 ? exp2_fast(x) : expf(x); }
+
+// Joins the parts that the warps of a tile hold and stores the tile's first `rows` rows at `to_o` and `to_ml`.  All warps of the CTA call it.
+template <typename E, int D>
 __device__ __forceinline__ void leave_tile(RowState<D>& st, float* join, int parts, int part, int tile, int lane, int rows, float* to_o, float* to_ml) {
     constexpr int P = D + 4;
     const int g = lane >> 2, t = lane & 3;
@@ -361,7 +496,7 @@ __device__ __forceinline__ void leave_tile(RowState<D>& st, float* join, int par
             for (int h = 0; h < 2; ++h) {
                 const float* row = from + (g + 8 * h) * P;
                 const float m2 = row[D], l2 = row[D + 1], m = fmaxf(st.m[h], m2), base = m == -INFINITY ? 0.f : m;
-                const float c1 = exp2_fast(st.m[h] - base), c2 = exp2_fast(m2 - base);
+                const float c1 = weight<E>(st.m[h] - base), c2 = weight<E>(m2 - base);
                 st.m[h] = m;
                 st.l[2 * h] = st.l[2 * h] * c1 + l2 * c2;
 #pragma unroll
@@ -385,30 +520,31 @@ __device__ __forceinline__ void leave_tile(RowState<D>& st, float* join, int par
 }
 
 // STAGES pages are in shared memory or on their way there.  A piece's parts are joined in the stage that was read last.
-template <int D, int STAGES>
-__global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __grid_constant__ BeamAttnArgs a) {
-    using T = BeamTile<D>;
+template <typename E, int D, int STAGES>
+__global__ void __launch_bounds__(kBaThreads, sizeof(E) == 4 || D <= 64 ? BeamTile<E, D>::kResident : 0) attention_beams_kernel(const __grid_constant__ BeamAttnArgs a) {
+    using T = BeamTile<E, D>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int tmp[kBaThreads / 16];
     __shared__ Unit ring[kBaRing];
     unsigned char* q_s = smem + STAGES * T::kStage;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int kvh = blockIdx.y, rep = a.n_heads / a.n_kv_heads;
-    float* turn_s = reinterpret_cast<float*>(q_s + a.sub_beams * rep * T::kPitchK);     // fused: [sequence of the part][cosines, sines of its D / 2 angles]
+    float* turn_s = reinterpret_cast<float*>(q_s + a.sub_beams * rep * T::kPitchQ);     // fused: [sequence of the part][cosines, sines of its D / 2 angles]
     Segment* seg = reinterpret_cast<Segment*>(turn_s + (a.inv_freq ? a.sub_beams * D : 0));
     int* lens = reinterpret_cast<int*>(seg + a.n_segments + 1);
     pdl_wait();
     // (only now: the kernel that joins the pieces may read a given plan as soon as it starts)
     pdl_launch_dependents();
     take_plan<kBaThreads>(a, seg, lens, tmp);
-    const int per = stretch_of(seg[a.n_segments].at, gridDim.x);
+    const int per = stretch_of(seg[a.n_segments], gridDim.x);
     const int2 mine = pages_before(a, seg, blockIdx.x * per, (blockIdx.x + 1) * per);
     const int u0 = mine.x, u1 = mine.y;
     if (u0 >= u1) return;
 
     const size_t page_elements = (size_t)a.n_kv_heads * kPageTokens * D, head_off = (size_t)kvh * kPageTokens * D;
     const uint32_t stage0 = (uint32_t)__cvta_generic_to_shared(smem), q_base = (uint32_t)__cvta_generic_to_shared(q_s);
-    constexpr int CK = D / 8, CV = kPageTokens / 8;        // 16-byte pieces of a row
+    constexpr bool kWide = sizeof(E) == 4;
+    constexpr int kEach = 16 / sizeof(E), CK = D / kEach, CV = kPageTokens / kEach;        // elements of 16 bytes, such pieces of a row
     auto know = [&](int u) {        // pages u .. u + 31 into the ring
         if (tid < kBaKnown && u + tid < u1) ring[(u + tid - u0) % kBaRing] = unit_of(a, seg, lens, u + tid);
     };
@@ -416,23 +552,23 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
         if (u < u1) {
             const Unit x = ring[(u - u0) % kBaRing];
             const uint32_t ks = stage0 + (uint32_t)(((u - u0) % STAGES) * T::kStage), vs = ks + kPageTokens * T::kPitchK;
-            const __nv_bfloat16* k = (const __nv_bfloat16*)a.k_pool + (size_t)x.page * page_elements + head_off;
-            const __nv_bfloat16* v = (const __nv_bfloat16*)a.v_pool + (size_t)x.page * page_elements + head_off;
+            const E* k = (const E*)a.k_pool + (size_t)x.page * page_elements + head_off;
+            const E* v = (const E*)a.v_pool + (size_t)x.page * page_elements + head_off;
             constexpr int RK = kBaThreads / CK, RV = kBaThreads / CV;
-            if (x.keys == kPageTokens && kBaThreads % CK == 0 && RK % 8 == 0) {   // a thread's pieces lie whole rows apart, at one place in them
+            if (x.keys == kPageTokens && kBaThreads % CK == 0 && RK % T::kPeriod == 0) {   // a thread's pieces lie whole rows apart, at one place in them
                 const uint32_t kt = ks + T::k_piece(tid / CK, tid % CK), vt = vs + T::v_piece(tid / CV, tid % CV);
-                k += tid * 8;
-                v += tid * 8;
+                k += tid * kEach;
+                v += tid * kEach;
 #pragma unroll
-                for (int i = 0; i < kPageTokens / RK; ++i) cp_async16(kt + i * RK * T::kPitchK, k + i * kBaThreads * 8);
+                for (int i = 0; i < kPageTokens / RK; ++i) cp_async16(kt + i * RK * T::kPitchK, k + i * kBaThreads * kEach);
 #pragma unroll
-                for (int i = 0; i < D / RV; ++i) cp_async16(vt + i * RV * T::kPitchV, v + i * kBaThreads * 8);
+                for (int i = 0; i < D / RV; ++i) cp_async16(vt + i * RV * T::kPitchV, v + i * kBaThreads * kEach);
             } else {
                 for (int i = tid; i < kPageTokens * CK; i += kBaThreads)
-                    cp_async16(ks + T::k_piece(i / CK, i % CK), k + (size_t)i * 8, i / CK < x.keys ? 16 : 0);
+                    cp_async16(ks + T::k_piece(i / CK, i % CK), k + (size_t)i * kEach, i / CK < x.keys ? 16 : 0);
                 // (values of positions past the sequence's end are read as zeros: a probability of 0 times what is not finite is not 0)
                 for (int i = tid; i < D * CV; i += kBaThreads)
-                    cp_async16(vs + T::v_piece(i / CV, i % CV), v + (size_t)i * 8, min(16, max(0, 2 * (x.keys - 8 * (i % CV)))));
+                    cp_async16(vs + T::v_piece(i / CV, i % CV), v + (size_t)i * kEach, min(16, max(0, (int)sizeof(E) * (x.keys - kEach * (i % CV)))));
             }
         }
         cp_async_commit();
@@ -444,6 +580,27 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
     };
     auto ask_queries = [&](int p) {     // of all rows of part p
         const int r0 = part_first_row(a, p);
+        if constexpr (kWide) {
+            const int n = part_rows(a, p) * rep * CK;
+            for (int c0 = tid; c0 < n; c0 += 4 * kBaThreads) {          // (four asked for at once)
+                float4 x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int c = min(c0 + k * kBaThreads, n - 1), row = c / CK, at = c % CK;
+                    x[k] = *reinterpret_cast<const float4*>((const E*)a.q + (size_t)(r0 + row / rep) * a.q_row_stride + (size_t)(kvh * rep + row % rep) * D + at * 4);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int c = c0 + k * kBaThreads, row = c / CK, at = c % CK;
+                    if (c >= n) continue;
+                    const Parts p0 = parts_of(x[k].x, x[k].y), p1 = parts_of(x[k].z, x[k].w);
+                    uint32_t* to = reinterpret_cast<uint32_t*>(q_s + row * T::kPitchQ + (at / 4) * 32 + (at % 4) * 4);
+                    to[0] = p0.h; to[T::kPlaneQ / 4] = p0.m; to[2 * T::kPlaneQ / 4] = p0.l;
+                    to[4] = p1.h; to[T::kPlaneQ / 4 + 4] = p1.m; to[2 * T::kPlaneQ / 4 + 4] = p1.l;
+                }
+            }
+            return;
+        } else {
         if (a.inv_freq) {
             const int n = part_rows(a, p);
             for (int c = tid; c < n * (D / 2); c += kBaThreads) {
@@ -478,22 +635,31 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
             cp_async16(q_base + T::k_piece(row, at), (const __nv_bfloat16*)a.q + (size_t)(r0 + row / rep) * a.q_row_stride
                                                          + (size_t)(kvh * rep + row % rep) * D + at * 8);
         }
+        }
     };
     know(u0);
     __syncthreads();
     int part_of = part_of_segment(a, ring[0].segment);
-    if (!a.inv_freq) ask_queries(part_of);               // (they arrive with the first page)
+    const bool made = kWide || a.inv_freq;
+    if (!made) ask_queries(part_of);                     // (they arrive with the first page)
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) issue(u0 + i);
-    if (a.inv_freq) ask_queries(part_of);                // (made while the first pages are on their way)
+    if (made) ask_queries(part_of);                      // (made while the first pages are on their way)
 
-    const float scale_log2 = 1.4426950408889634f / sqrtf((float)D);
+    const float scale = kWide ? 1.f / sqrtf((float)D) : 1.4426950408889634f / sqrtf((float)D);
     RowState<D> st;
-    uint32_t qa[D / 16][4];
+    uint32_t qa[kWide ? 1 : D / 16][4], q_row = 0;
     int segment = -1, parts = 1, part = 0, tile = warp, rows = 0, lo_max = 0, row_end = 0, row_lo[2] = {0, 0};
     auto leave = [&](int u) {           // behind page u - 1, with its stage to join in
         const size_t piece = (size_t)kvh * (gridDim.x + a.n_segments) + blockIdx.x + segment;
-        leave_tile<D>(st, reinterpret_cast<float*>(smem + ((u - 1 - u0) % STAGES) * T::kStage), parts, part, tile, lane, rows,
+        if constexpr (kWide) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                st.l[2 * h] += __shfl_xor_sync(0xffffffffu, st.l[2 * h], 1);
+                st.l[2 * h] += __shfl_xor_sync(0xffffffffu, st.l[2 * h], 2);
+            }
+        }
+        leave_tile<E, D>(st, reinterpret_cast<float*>(smem + ((u - 1 - u0) % STAGES) * T::kStage), parts, part, tile, lane, rows,
                       a.part_o + piece * kBaRows * D, a.part_ml + piece * kBaRows * 2);
     };
     for (int u = u0; u < u1; ++u) {
@@ -530,8 +696,12 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
             }
             // (rows behind the last one are its copies, and nothing of them is stored)
             const int row = min(tile * 16 + (lane & 15), rows - 1) + (i == 0 ? 0 : (i - 1) * rep);
+            if constexpr (kWide) {
+                q_row = q_base + row * T::kPitchQ;
+            } else {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) ldmatrix4(qa[ks], q_base + T::k_piece(row, ks * 2 + (lane >> 4)));
+                for (int ks = 0; ks < D / 16; ++ks) ldmatrix4(qa[ks], q_base + T::k_piece(row, ks * 2 + (lane >> 4)));
+            }
         }
         const int ahead = u + STAGES - 1;
         if (ahead < u1 && (ahead - u0) % kBaKnown == 0) {
@@ -539,7 +709,7 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
             __syncthreads();
         }
         issue(ahead);
-        if (a.write_cache && row_end - x.position <= kPageTokens) {      // a sequence's last page: its new key and value
+        if constexpr (!kWide) if (a.write_cache && row_end - x.position <= kPageTokens) {      // a sequence's last page: its new key and value
             const Segment own = seg[segment];
             const int slot = (u - u0) % STAGES, new_at = x.keys - 1, beam = own.row - part_first_row(a, part_of);
             const __nv_bfloat16* k_raw = (const __nv_bfloat16*)a.q + (size_t)own.row * a.q_row_stride + (size_t)(a.n_heads + kvh) * D;
@@ -566,12 +736,17 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
         if (tile * 16 < rows) {
             const uint32_t ks = stage0 + (uint32_t)(((u - u0) % STAGES) * T::kStage), vs = ks + kPageTokens * T::kPitchK;
             const bool masked = x.keys < kPageTokens || x.position < lo_max;
-            if (parts == 4) {
-                attend_keys<D, 16>(st, qa, ks, vs, part * 16, lane, scale_log2, masked, x.position, row_lo, row_end);
+            if constexpr (kWide) {
+                const unsigned char* page = smem + ((u - u0) % STAGES) * T::kStage;
+#pragma unroll 1
+                for (int first = part * 16; first < kPageTokens; first += parts * 16)
+                    attend_keys_f32<D>(st, q_row, page, page + kPageTokens * T::kPitchK, first, lane, scale, masked, x.position, row_lo, row_end);
+            } else if (parts == 4) {
+                attend_keys<D, 16>(st, qa, ks, vs, part * 16, lane, scale, masked, x.position, row_lo, row_end);
             } else {
 #pragma unroll 1
                 for (int first = part * 32; first < kPageTokens; first += parts * 32)
-                    attend_keys<D, 32>(st, qa, ks, vs, first, lane, scale_log2, masked, x.position, row_lo, row_end);
+                    attend_keys<D, 32>(st, qa, ks, vs, first, lane, scale, masked, x.position, row_lo, row_end);
             }
         }
     }
@@ -579,196 +754,11 @@ __global__ void __launch_bounds__(kBaThreads) attention_beams_kernel(const __gri
     leave(u1);
 }
 
-// float32, on multiply-adds.  Scores: a thread holds one key's dimensions in registers and takes every fourth row's query from shared memory
-// (one broadcast for four multiply-adds); output: it holds one dimension's 64 values and takes the probabilities of its rows.  Sums are
-// kept in four chains over the dimensions and four over the keys of a page, then a page's joins the row's.
-constexpr int kBfThreads = 256;
-template <int D>
-struct BeamTileF32 {
-    static constexpr int kPitchK = D + 4, kPitchV = kPageTokens + 4;       // floats: a multiple of 4, an odd number of 16 bytes
-    static constexpr int kStage = kPageTokens * kPitchK + D * kPitchV;
-    static constexpr int kStages = 2;
-    static constexpr int kQ = kBaRows * kPitchK, kScores = kBaRows * kPitchV, kState = 3 * kBaRows;
-    static constexpr int kBytes = 4 * (kStages * kStage + kQ + kScores + kState);
-    static constexpr int kRowGroups = kBfThreads / D;                       // of the output: so many rows at a time
-    static constexpr int kRowsEach = (kBaRows + kRowGroups - 1) / kRowGroups;
-};
-
-template <int D>
-__global__ void __launch_bounds__(kBfThreads) attention_beams_f32_kernel(const __grid_constant__ BeamAttnArgs a) {
-    using T = BeamTileF32<D>;
-    extern __shared__ __align__(16) float smem_f[];
-    __shared__ int tmp[kBfThreads / 16];
-    __shared__ Unit ring[kBaRing];
-    float* q_s = smem_f + T::kStages * T::kStage;
-    float* p_s = q_s + T::kQ;                       // [row][kPitchV] scores, then probabilities
-    float* m_s = p_s + T::kScores;
-    float* l_s = m_s + kBaRows;
-    float* f_s = l_s + kBaRows;                     // what a row's output so far is multiplied by
-    Segment* seg = reinterpret_cast<Segment*>(f_s + kBaRows);
-    int* lens = reinterpret_cast<int*>(seg + a.n_segments + 1);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int kvh = blockIdx.y, rep = a.n_heads / a.n_kv_heads;
-    pdl_wait();
-    pdl_launch_dependents();
-    take_plan<kBfThreads>(a, seg, lens, tmp);
-    const int per = stretch_of(seg[a.n_segments].at, gridDim.x);
-    const int2 mine = pages_before(a, seg, blockIdx.x * per, (blockIdx.x + 1) * per);
-    const int u0 = mine.x, u1 = mine.y;
-    if (u0 >= u1) return;
-
-    const size_t page_elements = (size_t)a.n_kv_heads * kPageTokens * D, head_off = (size_t)kvh * kPageTokens * D;
-    const uint32_t stage0 = (uint32_t)__cvta_generic_to_shared(smem_f);
-    auto know = [&](int u) {
-        if (tid < kBaKnown && u + tid < u1) ring[(u + tid - u0) % kBaRing] = unit_of(a, seg, lens, u + tid);
-    };
-    auto issue = [&](int u) {
-        if (u < u1) {
-            const Unit x = ring[(u - u0) % kBaRing];
-            const uint32_t ks = stage0 + (uint32_t)(((u - u0) % T::kStages) * T::kStage * 4), vs = ks + kPageTokens * T::kPitchK * 4;
-            const float* k = (const float*)a.k_pool + (size_t)x.page * page_elements + head_off;
-            const float* v = (const float*)a.v_pool + (size_t)x.page * page_elements + head_off;
-            constexpr int CK = D / 4, CV = kPageTokens / 4;
-#pragma unroll 4
-            for (int i = tid; i < kPageTokens * CK; i += kBfThreads) {
-                const int row = i / CK, c = i % CK;
-                cp_async16(ks + (row * T::kPitchK + c * 4) * 4, k + (size_t)row * D + c * 4, row < x.keys ? 16 : 0);
-            }
-#pragma unroll 4
-            for (int i = tid; i < D * CV; i += kBfThreads) {
-                const int row = i / CV, c = i % CV;
-                cp_async16(vs + (row * T::kPitchV + c * 4) * 4, v + (size_t)row * kPageTokens + c * 4, min(16, max(0, 4 * (x.keys - 4 * c))));
-            }
-        }
-        cp_async_commit();
-    };
-    know(u0);
-    __syncthreads();
-    issue(u0);
-
-    const float scale = 1.f / sqrtf((float)D);
-    const int key = tid % kPageTokens, score_group = tid / kPageTokens;
-    const int dim = tid % D, row_group = tid / D;
-    float o[T::kRowsEach];
-    int segment = -1, part_of = -1, rows = 0, q_row = 0, lo_max = 0, own_row = -1, r0 = 0;
-    auto leave = [&]() {
-        const size_t piece = (size_t)kvh * (gridDim.x + a.n_segments) + blockIdx.x + segment;
-        float* to = a.part_o + piece * kBaRows * D;
-        if (row_group < T::kRowGroups) {
-#pragma unroll
-            for (int j = 0; j < T::kRowsEach; ++j) {
-                const int r = row_group + j * T::kRowGroups;
-                if (r < rows) to[(size_t)r * D + dim] = o[j];
-            }
-        }
-        for (int r = tid; r < rows; r += kBfThreads)
-            *reinterpret_cast<float2*>(a.part_ml + (piece * kBaRows + r) * 2) = make_float2(m_s[r], l_s[r]);
-    };
-    for (int u = u0; u < u1; ++u) {
-        cp_async_wait<0>();
-        __syncthreads();
-        const int ahead = u + 1;
-        if (ahead < u1 && (ahead - u0) % kBaKnown == 0) {
-            know(ahead);
-            __syncthreads();
-        }
-        issue(ahead);
-        const Unit x = ring[(u - u0) % kBaRing];
-        if (x.segment != segment) {
-            if (segment >= 0) leave();
-            segment = x.segment;
-#pragma unroll
-            for (int j = 0; j < T::kRowsEach; ++j) o[j] = 0.f;
-            const int p = part_of_segment(a, segment), i = segment - p * (a.sub_beams + 1), n = part_rows(a, p);
-            r0 = part_first_row(a, p);
-            __syncthreads();        // (the rows' m and l, and the queries, have been read)
-            if (p != part_of) {
-                part_of = p;
-                constexpr int CQ = D / 4;
-                for (int c = tid; c < n * rep * CQ; c += kBfThreads) {
-                    const int row = c / CQ, at = c % CQ;
-                    const float* from = (const float*)a.q + (size_t)(r0 + row / rep) * a.q_row_stride + (size_t)(kvh * rep + row % rep) * D + at * 4;
-                    *reinterpret_cast<float4*>(q_s + row * T::kPitchK + at * 4) = *reinterpret_cast<const float4*>(from);
-                }
-            }
-            rows = i == 0 ? n * rep : rep;
-            q_row = i == 0 ? 0 : (i - 1) * rep;
-            own_row = i == 0 ? -1 : r0 + i - 1;
-            for (int r = tid; r < kBaRows; r += kBfThreads) { m_s[r] = -INFINITY; l_s[r] = 0.f; }
-            lo_max = 0;
-            if (i == 0) for (int b = 0; b < n; ++b) lo_max = max(lo_max, first_key(lens[r0 + b], a.window));
-            else lo_max = first_key(lens[own_row], a.window);
-            __syncthreads();
-        }
-        const float* k_tile = smem_f + ((u - u0) % T::kStages) * T::kStage;
-        const float* v_tile = k_tile + kPageTokens * T::kPitchK;
-        const bool masked = x.keys < kPageTokens || x.position < lo_max;
-        {
-            float4 k[D / 4];
-#pragma unroll
-            for (int c = 0; c < D / 4; ++c) k[c] = *reinterpret_cast<const float4*>(k_tile + key * T::kPitchK + c * 4);
-            for (int r = score_group; r < rows; r += kBfThreads / kPageTokens) {
-                const float* q = q_s + (q_row + r) * T::kPitchK;
-                float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll
-                for (int c = 0; c < D / 4; ++c) {
-                    const float4 v = *reinterpret_cast<const float4*>(q + c * 4);
-                    s0 += v.x * k[c].x; s1 += v.y * k[c].y; s2 += v.z * k[c].z; s3 += v.w * k[c].w;
-                }
-                float s = ((s0 + s1) + (s2 + s3)) * scale;
-                if (masked) {
-                    const int seq = own_row >= 0 ? own_row : r0 + r / rep, at = x.position + key;
-                    if (key >= x.keys || at < first_key(lens[seq], a.window)) s = -INFINITY;
-                }
-                p_s[r * T::kPitchV + key] = s;
-            }
-        }
-        __syncthreads();
-        for (int r = warp; r < rows; r += kBfThreads / 32) {
-            float* p = p_s + r * T::kPitchV;
-            const float s0 = p[lane], s1 = p[lane + 32], m0 = m_s[r], m = fmaxf(m0, warp_max(fmaxf(s0, s1)));
-            const float base = m == -INFINITY ? 0.f : m, e0 = expf(s0 - base), e1 = expf(s1 - base), sum = warp_sum(e0 + e1);
-            p[lane] = e0;
-            p[lane + 32] = e1;
-            __syncwarp();
-            if (lane == 0) {
-                const float f = expf(m0 - base);
-                f_s[r] = f;
-                l_s[r] = l_s[r] * f + sum;
-                m_s[r] = m;
-            }
-        }
-        __syncthreads();
-        if (row_group < T::kRowGroups) {
-            float4 v[kPageTokens / 4];
-#pragma unroll
-            for (int c = 0; c < kPageTokens / 4; ++c) v[c] = *reinterpret_cast<const float4*>(v_tile + dim * T::kPitchV + c * 4);
-#pragma unroll
-            for (int j = 0; j < T::kRowsEach; ++j) {
-                const int r = row_group + j * T::kRowGroups;
-                if (r < rows) {
-                    const float* p = p_s + r * T::kPitchV;
-                    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll
-                    for (int c = 0; c < kPageTokens / 4; ++c) {
-                        const float4 w = *reinterpret_cast<const float4*>(p + c * 4);
-                        s0 += w.x * v[c].x; s1 += w.y * v[c].y; s2 += w.z * v[c].z; s3 += w.w * v[c].w;
-                    }
-                    o[j] = o[j] * f_s[r] + ((s0 + s1) + (s2 + s3));
-                }
-            }
-        }
-    }
-    leave();
-}
-
 // A warp per (sequence, query head): the pieces that hold the row, first those of the shared pages, then of its own.  A lane reads a piece's maximum
 // and sum; the outputs are asked for eight pieces at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_constant__ BeamAttnArgs a, int n_ctas) {
     constexpr int E = D / 32, kAtOnce = 8;
-    // maxima are in units of log 2 where the scores were, in bfloat16
-    auto power = [](float x) { return sizeof(T) == 2 ? exp2_fast(x) : expf(x); };
     const int lane = threadIdx.x & 31, at = blockIdx.x * 4 + (threadIdx.x >> 5), rep = a.n_heads / a.n_kv_heads;
     const int seq = at / a.n_heads, head = at - seq * a.n_heads, kvh = head / rep, in_group = head - kvh * rep;
     const int g = seq / a.beams, beam = seq - g * a.beams, sub = a.n_sub == 1 ? 0 : beam / a.sub_beams, i = beam - sub * a.sub_beams;
@@ -780,8 +770,9 @@ __global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_
     int c0 = 0, n0 = 0, c1 = 0, n1 = 0;     // the first CTA with pages of the shared segment and their number; the same of its own
     if (mine) {
         const int2* of = reinterpret_cast<const int2*>(seg);        // (pages, at) of each
-        const int2 s0 = of[2 * shared], s1 = of[2 * shared + 2], o0 = of[2 * own], o1 = of[2 * own + 2], end = of[2 * a.n_segments];
-        const unsigned per = (unsigned)stretch_of(end.y, n_ctas), magic = per > 1 ? 0xffffffffu / per + 1u : 0u;
+        const int2 s0 = of[2 * shared], s1 = of[2 * shared + 2], o0 = of[2 * own], o1 = of[2 * own + 2];
+        const Segment end = seg[a.n_segments];
+        const unsigned per = (unsigned)stretch_of(end, n_ctas), magic = per > 1 ? 0xffffffffu / per + 1u : 0u;
         auto cta_of = [&](int x) {              // x / per
             if (magic == 0u) return x;
             const unsigned q = __umulhi((unsigned)x, magic);
@@ -789,7 +780,7 @@ __global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_
         };
         const int sa = s0.y + kSegmentCost, oa = o0.y + kSegmentCost, sn = s1.x - s0.x, on = o1.x - o0.x;
         c0 = cta_of(sa);
-        n0 = sn > 0 ? cta_of(sa + sn - 1) - c0 + 1 : 0;
+        n0 = sn > 0 ? cta_of(sa + ((sn - 1) << end.row)) - c0 + 1 : 0;
         c1 = cta_of(oa);
         n1 = on > 0 ? cta_of(oa + on - 1) - c1 + 1 : 0;
     }
@@ -806,7 +797,7 @@ __global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_
     for (int k0 = 0; k0 < n; k0 += 32) {
         float2 ml = make_float2(-INFINITY, 0.f);
         if (k0 + lane < n) ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * row_of(k0 + lane));
-        const float top = fmaxf(m, warp_max(ml.x)), zero = top == -INFINITY ? 0.f : top, keep = power(m - zero), f = power(ml.x - zero);
+        const float top = fmaxf(m, warp_max(ml.x)), zero = top == -INFINITY ? 0.f : top, keep = weight<T>(m - zero), f = weight<T>(ml.x - zero);
         l = l * keep + warp_sum(ml.y * f);
         m = top;
 #pragma unroll
@@ -848,7 +839,7 @@ static long long scratch_floats_of(int n_groups, int beams, int n_heads, int n_k
     return (segments + n_parts) * n_kv_heads * kBaRows * (head_dim + 2) + 4 * (segments + 1);
 }
 static int fill_args(BeamAttnArgs& a, const int* kv_lens, const int* shared_pages, int table_stride, int n_groups, int beams, int n_heads, int n_kv_heads,
-                     int window) {
+                     int window, int dtype) {
     if (beams < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads != 0 || window < 0 || table_stride < 1) return kErrBadArgument;
     const int rep = n_heads / n_kv_heads;
     if (rep > 16 || n_kv_heads > 65535) return kErrUnsupportedSize;
@@ -861,13 +852,14 @@ static int fill_args(BeamAttnArgs& a, const int* kv_lens, const int* shared_page
     a.n_parts = n_groups * a.n_sub; a.n_segments = (int)segments_of(n_groups, beams, rep);
     a.per_magic = (unsigned)(((1ull << 32) + a.sub_beams) / (a.sub_beams + 1));
     a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.window = window;
+    a.length = dtype == kF32 ? (a.sub_beams * rep > 32 ? 2 : a.sub_beams * rep > 16 ? 1 : 0) : 0;
     return 0;
 }
 
 constexpr int kSmShared = 228 * 1024, kCtaShared = 227 * 1024, kCtaReserved = 1024;      // bytes of an SM, the most of a CTA's, what each takes besides
 
 template <typename Kernel>
-static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int), int threads, int smem, int (&configured)[64], const BeamAttnArgs& a, int n_ctas,
+static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int), int smem, int (&configured)[64], const BeamAttnArgs& a, int n_ctas,
                         cudaStream_t stream) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
@@ -876,33 +868,34 @@ static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int), in
         if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
         configured[device] = smem;
     }
-    const int st = launch_pdl(kernel, dim3(n_ctas, a.n_kv_heads), dim3(threads), smem, stream, a);
+    const int st = launch_pdl(kernel, dim3(n_ctas, a.n_kv_heads), dim3(kBaThreads), smem, stream, a);
     if (st != 0) return st;
     const long long rows = (long long)a.n_seqs * a.n_heads;
     return launch_pdl(join, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, a, n_ctas);
 }
 
 // bytes of dynamic shared memory with that many stages
-template <int D>
+template <typename E, int D>
 static int beam_smem(const BeamAttnArgs& a, int stages) {
-    return stages * BeamTile<D>::kStage + a.sub_beams * ((a.n_heads / a.n_kv_heads) * BeamTile<D>::kPitchK + (a.inv_freq ? D * 4 : 0)) + plan_ints(a) * 4;
+    using T = BeamTile<E, D>;
+    return stages * T::kStage + a.sub_beams * ((a.n_heads / a.n_kv_heads) * T::kPitchQ + (a.inv_freq ? D * 4 : 0)) + plan_ints(a) * 4;
 }
 
+template <typename E, int D>
+static int launch_beams_of(const BeamAttnArgs& a, int n_ctas, cudaStream_t stream) {
+    using T = BeamTile<E, D>;
+    static int configured[2][64] = {};
+    constexpr int kStatic = 16 + kBaRing * (int)sizeof(Unit) + 1024;
+    const auto join = attention_beams_join_kernel<E, D>;
+    const int smem = beam_smem<E, D>(a, T::kMore), fewer = beam_smem<E, D>(a, 2);
+    if (smem + kStatic + kCtaReserved <= kSmShared / T::kResident)
+        return launch_beams(attention_beams_kernel<E, D, T::kMore>, join, smem, configured[0], a, n_ctas, stream);
+    if (fewer + kStatic > kCtaShared) return kErrUnsupportedSize;
+    return launch_beams(attention_beams_kernel<E, D, 2>, join, fewer, configured[1], a, n_ctas, stream);
+}
 template <int D>
 static int launch_beams_of(int dtype, const BeamAttnArgs& a, int n_ctas, cudaStream_t stream) {
-    static int configured[3][64] = {};
-    const auto join = dtype == kBF16 ? attention_beams_join_kernel<__nv_bfloat16, D> : attention_beams_join_kernel<float, D>;
-    if (dtype == kF32) {
-        const int smem = BeamTileF32<D>::kBytes + plan_ints(a) * 4;
-        if (smem + 2048 > kCtaShared) return kErrUnsupportedSize;
-        return launch_beams(attention_beams_f32_kernel<D>, join, kBfThreads, smem, configured[0], a, n_ctas, stream);
-    }
-    // As many stages as leave room for three CTAs an SM with heads of up to 64, two with wider ones.
-    constexpr int kMore = D <= 64 ? 4 : 3, kResident = D <= 64 ? 3 : 2, kStatic = 16 + kBaRing * (int)sizeof(Unit);
-    const int smem = beam_smem<D>(a, kMore);
-    if (smem + kStatic + kCtaReserved <= kSmShared / kResident)
-        return launch_beams(attention_beams_kernel<D, kMore>, join, kBaThreads, smem, configured[1], a, n_ctas, stream);
-    return launch_beams(attention_beams_kernel<D, 2>, join, kBaThreads, beam_smem<D>(a, 2), configured[2], a, n_ctas, stream);
+    return dtype == kF32 ? launch_beams_of<float, D>(a, n_ctas, stream) : launch_beams_of<__nv_bfloat16, D>(a, n_ctas, stream);
 }
 
 }  // namespace b200
@@ -921,12 +914,13 @@ extern "C" int b200_attention_beams_plan_ints(int n_groups, int beams, int n_hea
 // The plan alone, for the layers of a step that share lengths, shared pages, heads and window.  fresh: 1 for the fused variant that writes the
 // cache (the page that holds the last position is then no shared one, whatever shared_pages says).
 extern "C" int b200_attention_beams_plan(int* plan, const int* kv_lens, const int* shared_pages, int table_stride, int n_groups, int beams, int n_heads,
-                                         int n_kv_heads, int window, int fresh, cudaStream_t stream) {
+                                         int n_kv_heads, int window, int dtype, int fresh, cudaStream_t stream) {
     using namespace b200;
     if (n_groups <= 0) return 0;
     BeamAttnArgs a;
-    const int st = fill_args(a, kv_lens, shared_pages, table_stride, n_groups, beams, n_heads, n_kv_heads, window);
+    const int st = fill_args(a, kv_lens, shared_pages, table_stride, n_groups, beams, n_heads, n_kv_heads, window, dtype);
     if (st != 0) return st;
+    if (dtype != kF32 && dtype != kBF16) return kErrBadArgument;
     if (((uintptr_t)plan & 15) != 0) return kErrUnsupportedSize;
     a.plan = plan;
     a.fresh = fresh != 0;
@@ -950,7 +944,7 @@ static int attention_beams(const void* q, long long q_row_stride, void* out, con
                            int write_cache, cudaStream_t stream) {
     if (n_groups <= 0) return 0;
     BeamAttnArgs a;
-    const int st = fill_args(a, kv_lens, shared_pages, table_stride, n_groups, beams, n_heads, n_kv_heads, window);
+    const int st = fill_args(a, kv_lens, shared_pages, table_stride, n_groups, beams, n_heads, n_kv_heads, window, dtype);
     if (st != 0) return st;
     if ((dtype != kF32 && dtype != kBF16) || n_parts < 1 || pairing < 0 || pairing > 1) return kErrBadArgument;
     if (head_dim % 32 != 0 || head_dim < 32 || head_dim > 128 || n_parts > 65535 || (long long)a.n_seqs * n_heads > (1 << 28)) return kErrUnsupportedSize;

@@ -8,9 +8,14 @@
 // CTAs does not matter.
 //
 // Pages: a CTA takes a head of an entry of one source.  Its keys are one run of bytes (positions follow one another), its values head_dim rows of
-// 64 positions of which the first n are taken; 16 bytes an access, four of the keys and four of the values a thread asked for before the first
-// is stored.  States: a CTA takes 2,048 accesses (of the widest that the addresses allow) of one state, eight a thread.  Bound by HBM, and
-// where pages are not full by the sectors that rows of values end in: they are read to be written.
+// 64 positions of which the first n are taken; 16 bytes an access, two of the keys, two of the values and two of the values' ends a thread asked
+// for before the first is stored (four of each take 96 registers, half the CTAs, and are no faster).  States: a CTA takes 2,048 accesses (of the
+// widest that the addresses allow) of one state, eight a thread.
+//
+// Bound by HBM, and where pages are not full by the sectors that rows of values end in: they are read to be written.  Measured: 40 pages of
+// 1 to 64 positions in 32 layers of 8 heads of 128, bfloat16, 81 us: 449 MB move (5.6 TB/s) where 260 MB are asked for; pages filled to a
+// multiple of 16 positions run at 5 to 6.3 TB/s of what is asked for.  19 states of 2.4 MB to 37
+// places, 134 MB, 23.5 us, 5.7 TB/s.
 #include "common.cuh"
 
 namespace b200 {

@@ -100,7 +100,7 @@ def _beam_launch(ctx, page_table, cache, mixer, dtype, writes_cache: bool):
     plan = ctx.extras.get(key)
     if plan is None:
         plan = ctx.extras[key] = ops.attention_beams_plan(ctx.kv_lens, shared, page_table.shape[1], mixer.n_heads, mixer.n_kv_heads,
-                                                          mixer.window or 0, writes_cache=writes_cache)
+                                                          mixer.window or 0, writes_cache=writes_cache, dtype=dtype)
     return shared, parts, plan
 
 

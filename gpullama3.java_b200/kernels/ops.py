@@ -181,7 +181,7 @@ _SIGNATURES = {
     "b200_attention_beams_rope": ("attention_beams", [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                                       c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_int, c_int,
                                                       c_int, c_void_p, c_void_p, c_int, c_int]),
-    "b200_attention_beams_plan": ("attention_beams", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "b200_attention_beams_plan": ("attention_beams", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "b200_sample_rows": ("sampling", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_float, c_void_p]),
 }
 
@@ -1313,9 +1313,9 @@ _beams_sizes: dict = {}
 
 
 def attention_beams_plan(kv_lens: torch.Tensor, shared_pages: torch.Tensor, table_width: int, n_heads: int, n_kv_heads: int, window: int,
-                         out: torch.Tensor | None = None, *, writes_cache: bool = False) -> torch.Tensor:
+                         out: torch.Tensor | None = None, *, writes_cache: bool = False, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """How the pages of a step's groups are shared out (int32), for several calls of ``attention_decode_beams`` in that step, or with
-    ``writes_cache`` of ``attention_decode_beams_rope``."""
+    ``writes_cache`` of ``attention_decode_beams_rope``.  ``dtype``: of the calls, for which the shares are made equal."""
     _here(kv_lens, shared_pages, out)
     n_seqs, n_groups = kv_lens.numel(), shared_pages.numel()
     assert kv_lens.dtype == shared_pages.dtype == torch.int32 and kv_lens.is_contiguous() and shared_pages.is_contiguous()
@@ -1326,8 +1326,8 @@ def attention_beams_plan(kv_lens: torch.Tensor, shared_pages: torch.Tensor, tabl
         out = torch.empty(need, dtype=torch.int32, device=kv_lens.device)
     assert out.dtype == torch.int32 and out.is_contiguous() and out.numel() >= need
     _check(_fn("b200_attention_beams_plan")(out.data_ptr(), kv_lens.data_ptr(), shared_pages.data_ptr(), int(table_width), n_groups,
-                                            n_seqs // n_groups, n_heads, n_kv_heads, int(window), 1 if writes_cache else 0, _stream()),
-           "attention_beams_plan")
+                                            n_seqs // n_groups, n_heads, n_kv_heads, int(window), dtype_code(dtype), 1 if writes_cache else 0,
+                                            _stream()), "attention_beams_plan")
     return out
 
 
