@@ -14,12 +14,11 @@
 // of the first tile reach, so that few logits beyond `keep` are ever listed, and rises when the list is cut down; a thread of a later tile
 // compares its sixteen logits' maximum once and mostly goes on.  So a chunk costs the reading, an exponential a logit, and a few
 // searches of 32 steps with a barrier each.  (Lists of each warp by itself need no barriers, but then every warp holds `keep`
-// candidates of its own and the ordering at the end is of eight times as many: 2.5 times as long with 64 kept.)
+// candidates of its own and the ordering at the end is of eight times as many, which took longer than all the rest.)
 //
 // Exponentials are taken in 32 bits, relative to a whole number, added in 32 bits over eight of a thread's logits and in 64 from there on: a
-// row's lse is off by about 2e-8 of itself, as 64-bit totals of the plain form's 32-bit logarithms are, and totals are compared in 64
-// bits, so that two beams' continuations change places only where they are that near to each other.  A score is rounded to 32 bits
-// once, when it is stored.
+// row's lse is off by about 2e-8 of itself (measured against 64 bits), and totals are compared in 64 bits, so that two beams'
+// continuations change places only where they are that near to each other.  A score is rounded to 32 bits once, when it is stored.
 //
 // Bound by: HBM in bytes (4 per logit), in fact by the rows' instructions and the merge's chain of barriers.  Measured: 64 rows of
 // 128,256 logits, 16 kept each of 8, 18.8 us of which the reading needs 5.0; 256 rows, 64 kept, 46.6 us of 20.0 (rows 39 us at 3.4 TB/s,

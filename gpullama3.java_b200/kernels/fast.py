@@ -74,16 +74,25 @@ def beams_share_attention(ctx, mixer, dtype, capacity: int) -> bool:
     """Whether a decode step's attention reads the pages that a group's sequences share once for all of them: a beam search's step of a
     mixer whose mask is causality and at most a window, where that is faster.  ``capacity``: the longest sequence the step must be right for.
 
-    Up to 16 sequences the products of a step stream through L1, and the attention of groups, which keeps its pages in shared memory, makes every
-    SM change its split twice a layer; beyond that the separate sequences' kernel is faster while they are short, for their pages are
-    in L2 for all but the first of a group.  A step in ms, of groups / of separate sequences: 1B shape 4 beams at 1,000 positions 1.02 / 0.74;
+    bfloat16: up to 16 sequences the products of a step stream through L1, and the attention of groups, which keeps its pages in shared memory,
+    makes every SM change its split twice a layer; beyond that the separate sequences' kernel is faster while they are short, for their pages
+    are in L2 for all but the first of a group.  A step in ms, of groups / of separate sequences: 1B shape 4 beams at 1,000 positions 1.02 / 0.74;
     5 x 4 at 450 0.98 / 0.95, at 900 0.99 / 1.01, at 1,900 1.05 / 1.13; 8 x 8 at 450 1.22 / 1.16, at 900 1.24 / 1.27, at 4,000 1.42 / 1.98;
-    32 x 2 at 900 1.37 / 1.30, at 1,900 1.52 / 1.58; 8B shape 8 x 8 at 220 4.55 / 4.45, at 900 4.63 / 5.21, at 3,000 5.03 / 7.92; 1B in float32
-    8 x 4 at 900 3.11 / 3.11, at 1,900 3.36 / 3.73."""
+    32 x 2 at 900 1.37 / 1.30, at 1,900 1.52 / 1.58; 8B shape 8 x 8 at 220 4.55 / 4.45, at 900 4.63 / 5.21, at 3,000 5.03 / 7.92.
+
+    float32: faster as soon as there is enough to read, whatever the number of sequences.  1B shape: 1 x 4 at 900 1.51 / 1.45; 1 x 8 at 1,900 1.99 /
+    2.06; 4 x 4 at 450 2.66 / 2.57, at 900 2.69 / 2.73, at 3,900 2.87 / 3.92; 8 x 4 at 200 2.72 / 2.71, at 450 2.78 / 2.84; 8 x 8 at 200
+    2.98 / 2.99, at 1,900 3.38 / 5.08, at 3,900 3.73 / 7.44."""
     beams = getattr(ctx, "beams", 1)
-    return (beams > 1 and ctx.all_decode and not (mixer.keep_first or getattr(mixer, "has_terms", False) or getattr(mixer, "chunk", None))
-            and ctx.n_seqs > 16 and min(capacity, mixer.window or capacity) >= 1024 and beams * capacity >= 4096
-            and ops.attention_beams_supported(dtype, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim))
+    if beams == 1 or not ctx.all_decode or mixer.keep_first or getattr(mixer, "has_terms", False) or getattr(mixer, "chunk", None):
+        return False
+    seen = min(capacity, mixer.window or capacity)
+    if dtype == torch.float32:
+        enough = ctx.n_seqs * seen >= 16384
+    else:
+        enough = ctx.n_seqs > 16 and seen >= 1024 and beams * capacity >= 4096
+    return (enough and ops.attention_beams_supported(dtype, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim)
+            and ops.attention_beams_takes(ctx.n_seqs // beams, beams, mixer.n_heads, mixer.n_kv_heads))
 
 
 def _capacity(ctx, cache) -> int:

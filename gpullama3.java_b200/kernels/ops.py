@@ -1285,6 +1285,14 @@ def attention_beams_supported(dtype: torch.dtype, n_heads: int, n_kv_heads: int,
     return dtype in _DTYPE_CODE and head_dim in (32, 64, 96, 128) and n_heads % n_kv_heads == 0 and n_heads // n_kv_heads <= 16
 
 
+def attention_beams_takes(n_groups: int, beams: int, n_heads: int, n_kv_heads: int) -> bool:
+    """Whether one call takes so many groups: 2,048 stretches of pages (a group's shared ones, in parts of at most 64 rows to a kv head, and each
+    sequence's own; attention_beams.cu) fit a CTA's shared memory."""
+    rep = n_heads // n_kv_heads
+    sub = min(-(-beams // -(-beams * rep // 64)), 64 // rep)
+    return n_groups * -(-beams // sub) * (sub + 1) <= 2048
+
+
 def attention_beams_parts(n_groups: int, beams: int, n_heads: int, n_kv_heads: int, head_dim: int, capacity: int, dtype: torch.dtype,
                           device) -> int:
     """How many CTAs of a kv head share the pages of a step's groups: as many as the GPU holds at once, no more than there may be
@@ -1339,6 +1347,8 @@ def _beams_checked(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_
         raise KernelError(f"attention_decode_beams: {n_heads} heads on {n_kv_heads} of {head_dim} in {q.dtype}")
     if n_groups == 0 or n_seqs % n_groups:
         raise KernelError(f"{n_seqs} sequences do not make {n_groups} equal groups")
+    if not attention_beams_takes(n_groups, n_seqs // n_groups, n_heads, n_kv_heads):
+        raise KernelError(f"attention_decode_beams: {n_groups} groups of {n_seqs // n_groups} are more than one call takes")
     assert q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and out.is_contiguous() and out.shape[1] == n_heads * head_dim
     assert q.shape[0] >= n_seqs and q.stride(-1) == 1
     assert kv_lens.dtype == page_table.dtype == shared_pages.dtype == torch.int32

@@ -245,3 +245,20 @@ def test_forked_sequences_go_on_by_ordinary_steps(session_tmp, family, name):
     cache.check_invariants()
     for s in cache.live_slots():
         cache.release(s)
+
+
+def test_more_groups_than_one_attention_call_takes(session_tmp):
+    """Such a step reads every sequence for itself: the same as in smaller batches."""
+    from gpullama3.java_b200.engine.api import Engine
+    from gpullama3.java_b200.kernels import ops
+
+    cfg_json, norm_std = TINY["B"]
+    d = make_model_dir(session_tmp, cfg_json, seed=21, norm_std=norm_std, scale=SCALE)
+    prompts = random_prompts(cfg_json["vocab_size"], [1 + i % 3 for i in range(260)], seed=9)
+    H, KVH = cfg_json["num_attention_heads"], cfg_json["num_key_value_heads"]
+    assert not ops.attention_beams_takes(260, 8, H, KVH) and ops.attention_beams_takes(32, 8, H, KVH)
+    found = [Engine.from_folder(d, dtype="float32", max_tokens=64 * 2100, max_batch=n).beam_search(prompts, 8, 3, stop_ids=(), return_hypotheses=True)
+             for n in (8 * 260, 8 * 32)]
+    # (other kernels for other numbers of rows: the same tokens but where two scores are as near as float32 is)
+    for a, b in zip(*found):
+        assert a.tokens == b.tokens or abs(a.log_prob - b.log_prob) <= 1e-4 * len(a.tokens)
