@@ -374,7 +374,8 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const uint32_t (&qa
 
 // float32: x = h + m + l, three bfloat16 numbers of 8 bits each (what is left is below 2^-26 of x); a product is h h + (h m + m h) + (m m + h l + l h),
 // six on the tensor cores with an error below that of one product's rounding.  The three magnitudes are added separately, and the output of 16
-// keys before it joins the row's, in 32 bits: a tensor core's own sum drops bits instead of rounding them.
+// keys before it joins the row's, in 32 bits: a tensor core's own sum drops bits instead of rounding them.  Numbers from 2^-109 to 2^127 have all three
+// parts; what is not finite gives NaN.
 struct Parts {
     uint32_t h, m, l;
 };

@@ -488,3 +488,35 @@ def test_fused_rotation_and_cache_write(shared, lens, H, KVH, D, window, write_c
     again.zero_()
     ops.attention_decode_beams(rotated, rotated.shape[1], again, one.lens, one.table, fewer, one.k, one.v, H, KVH, D, window, parts, plan=plain_plan)
     assert torch.equal(again, want)
+
+
+@pytest.mark.parametrize("case", [4, 5, 6, 7, 9])
+@pytest.mark.parametrize("window", [0, 130])
+def test_float32_attention_takes_any_plan_of_its_groups(case, window):
+    """A plan shares the work out for one type; a call of the other takes it all the same: sums are cut elsewhere, nothing is left out."""
+    shared, lens, H, KVH, D = SHAPES[case]
+    groups = Groups(shared, lens, H, KVH, D, torch.float32, seed=case)
+    out = torch.empty(len(lens), H * D, device="cuda")
+    for parts in (2, 7, 30):
+        direct = groups.run(window, parts)
+        for dtype in (torch.float32, torch.bfloat16):
+            plan = ops.attention_beams_plan(groups.lens, groups.shared, groups.width, H, KVH, window, dtype=dtype)
+            ops.attention_decode_beams(groups.q, groups.q.stride(0), out, groups.lens, groups.table, groups.shared, groups.k, groups.v, H, KVH, D,
+                                       window, parts, plan=plan)
+            if dtype == torch.float32:
+                assert torch.equal(out, direct)
+            else:       # the same products in another order of sums: each within the bound of `check`, so within twice that of each other
+                assert float((out - direct).norm() / direct.norm()) <= 2 * (80 + 2 * groups.width) * HALF_STEP
+        groups.check(window, parts)
+
+
+@pytest.mark.parametrize("power", [-60, -20, 40, 100])
+def test_float32_attention_of_scaled_numbers_keeps_its_bits(power):
+    """Powers of two go through every part and product unchanged: keys by 2^power and queries by 2^-power, and values by 2^power."""
+    groups = Groups([3, 2], [250, 230, 200, 192, 140, 170], 8, 2, 64, torch.float32)
+    want = groups.run()
+    groups.k *= 2.0 ** power
+    groups.q = groups.q * 2.0 ** -power
+    assert torch.equal(groups.run(), want)
+    groups.v *= 2.0 ** (power - 10)
+    assert torch.equal(groups.run(), want * 2.0 ** (power - 10))
