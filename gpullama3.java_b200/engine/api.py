@@ -132,7 +132,7 @@ class Engine:
                     n_best: int = 1, stop_ids=None, return_hypotheses: bool = False):
         """The most probable continuation found per prompt with ``beams`` beams (token ids, the stop token included when one ended it); with
         ``n_best`` > 1 a list of so many per prompt, the best first.  Hypotheses are ranked by the sum of their tokens' log
-        probabilities over their length to the power of ``length_penalty``.  ``return_hypotheses``: ``BeamHypothesis`` records, with
+        probabilities over their length to the power of ``length_penalty`` (at most 32 up or down).  ``return_hypotheses``: ``BeamHypothesis`` records, with
         log probability, score and finish reason, in place of token ids.  A batch takes ``beams`` sequences of ``max_batch``
         per request."""
         if stop_ids is None:

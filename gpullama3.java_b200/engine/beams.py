@@ -38,8 +38,8 @@ class BeamParams:
             raise ValueError(f"a beam search needs at least one beam, got {self.beams}")
         if not 1 <= self.n_best <= self.beams:
             raise ValueError(f"n_best {self.n_best} must be within [1, {self.beams}]")
-        if not math.isfinite(self.length_penalty):
-            raise ValueError("length_penalty must be finite")
+        if not -32 <= self.length_penalty <= 32:        # (a length to that power is a number)
+            raise ValueError(f"length_penalty must be within [-32, 32], got {self.length_penalty}")
 
 
 @dataclass

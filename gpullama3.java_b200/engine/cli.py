@@ -124,6 +124,8 @@ def main(argv=None) -> int:
         parser.error("--suffix: fill-in-the-middle is not part of this library")
     if args.beams < 1:
         parser.error("--beams must be at least 1")
+    if not -32 <= args.length_penalty <= 32:
+        parser.error("--length-penalty must be within [-32, 32]")
     if args.beams > args.max_batch:
         parser.error(f"--beams {args.beams} needs --max-batch {args.beams} at least")
     if args.temperature < 0:

@@ -430,3 +430,18 @@ def test_attention_parts_follow_the_gpu_and_the_pages():
         assert parts(8, 8, 32, 8, 64, 4352, torch.bfloat16, "cuda") <= 3 * 148 // 8
         assert parts(1, 1, 1, 1, 32, 1, torch.float32, "cuda") == 2
         assert parts(4, 2, 256, 256, 128, 100000, torch.bfloat16, "cuda") >= 1
+
+
+@pytest.mark.parametrize("penalty", [400.0, -400.0, 33.0, float("inf"), float("nan")])
+def test_length_penalties_without_a_score_are_refused(penalty):
+    """A length to such a power is no number, or 0."""
+    with pytest.raises(ValueError, match="length_penalty"):
+        BeamParams(2, penalty)
+
+
+@pytest.mark.parametrize("penalty", [32.0, -32.0])
+def test_the_largest_length_penalties_have_scores(penalty):
+    request = BeamRequest(BeamParams(2, penalty), 5, 1 << 20, 1 << 21, frozenset({7}))
+    request.beams = [([1] * ((1 << 20) - 2), -3.0), ([2] * ((1 << 20) - 2), -4.0)]
+    request.advance([(-3.5, 0, 7), (-4.5, 1, 7), (-5.0, 0, 1), (-6.0, 1, 1)])
+    assert all(math.isfinite(h.score) for h in request.finished) and len(request.finished) == 2
