@@ -130,11 +130,11 @@ class Engine:
 
     def beam_search(self, prompts: list[list[int]], beams: int = 4, max_new_tokens: int = 16, *, length_penalty: float = 1.0,
                     n_best: int = 1, stop_ids=None, return_hypotheses: bool = False):
-        """The most probable continuation found per prompt with ``beams`` beams (token ids, the stop token included when one ended it); with
-        ``n_best`` > 1 a list of so many per prompt, the best first.  Hypotheses are ranked by the sum of their tokens' log
-        probabilities over their length to the power of ``length_penalty`` (at most 32 up or down).  ``return_hypotheses``: ``BeamHypothesis`` records, with
-        log probability, score and finish reason, in place of token ids.  A batch takes ``beams`` sequences of ``max_batch``
-        per request."""
+        """The most probable continuation found per prompt with ``beams`` beams (token ids, the stop token included when one ended
+        it); with ``n_best`` > 1 a list of so many per prompt, the best first.  Hypotheses are ranked by the sum of their tokens'
+        log probabilities over their length to the power of ``length_penalty`` (at most 32 up or down).  ``return_hypotheses``:
+        ``BeamHypothesis`` records, with log probability, score and finish reason, in place of token ids.  A batch takes
+        ``beams`` sequences of ``max_batch`` per request."""
         if stop_ids is None:
             stop_ids = self.stop_ids
         found = self.searcher.search([list(p) for p in prompts], max_new_tokens, BeamParams(beams, length_penalty, n_best), stop_ids)
