@@ -108,6 +108,16 @@ class CacheGroup:
         """Raise CacheError if the group's bookkeeping is inconsistent."""
 
 
+def common_entries(a: list[int], b: list[int]) -> int:
+    """How many first entries of two rows of pages are the same.  Rows of sequences that began as one mostly differ at their ends."""
+    n = min(len(a), len(b))
+    while n and a[n - 1] != b[n - 1]:
+        n -= 1
+    if a[:n] != b[:n]:
+        n = next(i for i in range(n) if a[i] != b[i])
+    return n
+
+
 class PagedGroup(CacheGroup):
     """Bookkeeping of a group that grows page by page; subclasses own the device storage and the view."""
     paged = True
@@ -159,6 +169,15 @@ class PagedGroup(CacheGroup):
         self.pool.share([p for p in row if p >= 0])
         self.rows[new_slot] = row
         self._changed(new_slot)
+
+    def refork(self, slot: int, over: int, length: int) -> None:
+        """The same in place of the sequence in ``over``, which is over: pages that it has in common with ``slot`` stay its own."""
+        row, old = self.rows[slot][:pages_for(length)], self.rows[over]
+        n = common_entries(row, old)
+        self.pool.share([p for p in row[n:] if p >= 0])
+        self.pool.free([p for p in old[n:] if p >= 0])
+        self.rows[over] = row
+        self._changed(over)
 
     def shared_writes(self, slots, lengths: dict[int, int]) -> int:
         """How many pages must be copied before all of ``slots`` (each once) are written to behind their lengths."""
@@ -420,13 +439,23 @@ class SequenceCache:
         for child, p in enumerate(parents):
             if p not in keeper or child == p:
                 keeper[p] = child
-        if len(keeper) < len(parents):
-            self._check_can_fork()
-        for p, slot in enumerate(slots):
-            if p not in keeper:
-                self.release(slot)
+        over = [slot for p, slot in enumerate(slots) if p not in keeper]
         others = [child for child, p in enumerate(parents) if keeper[p] != child]
-        new = dict(zip(others, self.fork([slots[parents[child]] for child in others])))
+        if others:
+            self._check_can_fork()
+        new = {}
+        for child in others:    # in the place of a sequence that is over: there are as many at least
+            slot, taken = slots[parents[child]], over.pop()
+            new[child] = taken
+            self.ownership_changes += 1
+            self._length[taken] = self._length[slot]
+            for g in self.paged_groups:
+                g.refork(slot, taken, self._length[slot])
+        if others:
+            for g in self.slot_groups:
+                g.copy([(slots[parents[child]], new[child]) for child in others])
+        for slot in over:
+            self.release(slot)
         return [new[child] if child in new else slots[p] for child, p in enumerate(parents)]
 
     def shared_pages(self, slots: list[int]) -> list[int]:

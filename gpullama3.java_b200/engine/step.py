@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from ..cache.pages import PAGE_TOKENS
-from ..cache.sequence_cache import SequenceCache
+from ..cache.sequence_cache import SequenceCache, common_entries
 from ..parts.base import StepContext
 from .workspace import Workspace
 
@@ -172,7 +172,8 @@ class DecodeGraph:
         self.last_slots: list[int] | None = None
         self.last_pos: list[int] | None = None
         self.last_owners = -1                         # the cache's ownership count at the last refresh
-        self.row_stamps: list[list] = []              # of a beam search's step: which rows of pages the staging buffer holds
+        self.row_stamps: list[list] = []              # of a beam search's step: which rows of pages the staging buffer holds, and the rows
+        self.rows_held: list[list] = []
         # the step is replayed for every length its page tables can address: parts shape their launches for that
         self.kv_capacity = [w * PAGE_TOKENS for w in widths]
 
@@ -214,19 +215,21 @@ class DecodeGraph:
         if not self.row_stamps:
             pieces, _, _ = _pack(self.cache, slots, start_pos, [[t] for t in tokens], list(range(n)), self.widths)
             np.concatenate(pieces, out=h[:self.shared_offset])
-            self.row_stamps = [[None] * n for _ in groups]
+            self.row_stamps = [[g.stamp(s) for s in slots] for g in groups]
+            self.rows_held = [[list(g.rows[s]) for s in slots] for g in groups]
         else:
             h[0:n] = tokens
             h[n:2 * n] = start_pos
             h[4 * n + 1:5 * n + 1] = h[n:2 * n] + 1
             h[5 * n + 1:6 * n + 1] = slots
-        for g, stamps, off, w in zip(groups, self.row_stamps, self.table_offsets, self.widths):
+        for g, stamps, held, off, w in zip(groups, self.row_stamps, self.rows_held, self.table_offsets, self.widths):
             for i, s in enumerate(slots):
                 stamp = g.stamp(s)
                 if stamps[i] != stamp:
                     row = g.rows[s]
-                    h[off + i * w: off + i * w + len(row)] = np.maximum(np.asarray(row, dtype=np.int32), 0)
-                    stamps[i] = stamp
+                    for j in range(common_entries(row, held[i]), len(row)):
+                        h[off + i * w + j] = max(row[j], 0)
+                    stamps[i], held[i] = stamp, list(row)
         h[self.shared_offset:self.uniform_offset] = _shared_pages(self.cache, slots, self.beams)
         h[self.uniform_offset:self.uniform_offset + n] = np.asarray(scores, dtype=np.float32).view(np.int32)
 

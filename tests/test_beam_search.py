@@ -445,3 +445,36 @@ def test_the_largest_length_penalties_have_scores(penalty):
     request.beams = [([1] * ((1 << 20) - 2), -3.0), ([2] * ((1 << 20) - 2), -4.0)]
     request.advance([(-3.5, 0, 7), (-4.5, 1, 7), (-5.0, 0, 1), (-6.0, 1, 1)])
     assert all(math.isfinite(h.score) for h in request.finished) and len(request.finished) == 2
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_reordered_rows_are_the_parents_with_windows_too(seed):
+    """A child in the place of a sequence that is over keeps the pages they have in common: rows, holders and lengths come out as its parent's."""
+    rng = random.Random(seed)
+    c = SequenceCache({0: KVCacheNeed(1, 16), 1: KVCacheNeed(1, 16, window=100), 2: StateNeed((3,), torch.float32)}, max_tokens=64 * 80, max_slots=6,
+                      dtype=torch.float32, device="cpu", window_slack=64)
+    slots = [c.acquire()]
+    c.reserve([(slots[0], 70)])
+    c.commit(slots[0], 70)
+    slots += c.fork([slots[0]] * 5)
+    state, = c.slot_groups
+    for step in range(300):
+        new = [1] * len(slots) if rng.random() < 0.8 else [rng.randint(1, 40) for _ in slots]      # equally long, and not
+        try:
+            c.reserve(list(zip(slots, new)))
+        except CacheFull:
+            for s in slots:
+                c.release(s)
+            slots = [c.acquire()]
+            slots += c.fork([slots[0]] * 5)
+            continue
+        for s, n in zip(slots, new):
+            c.commit(s, n)
+            state.data[:, s] = float(step * 10 + s)
+        parents = [rng.randrange(len(slots)) for _ in slots]
+        want = [([g.rows[slots[p]][:pages_for(c.length(slots[p]))] for g in c.paged_groups], c.length(slots[p]), state.data[:, slots[p]].clone())
+                for p in parents]
+        slots = c.reorder(slots, parents)
+        for s, (rows, length, kept) in zip(slots, want):
+            assert [g.rows[s][:pages_for(length)] for g in c.paged_groups] == rows and c.length(s) == length and torch.equal(state.data[:, s], kept)
+        c.check_invariants()
