@@ -179,33 +179,32 @@ class PagedGroup(CacheGroup):
         self.rows[over] = row
         self._changed(over)
 
-    def shared_writes(self, slots, lengths: dict[int, int]) -> int:
-        """How many pages must be copied before all of ``slots`` (each once) are written to behind their lengths."""
-        writers: dict[int, int] = {}
+    def shared_writes(self, slots, lengths: dict[int, int]) -> tuple[list[tuple[int, int]], int]:
+        """Of ``slots`` (each once) those that are about to write into a page that has other holders, with the page, and how many pages must be
+        copied before they do (the last holder of a page writes into it)."""
+        writers, times = [], {}
+        holders, rows = self.pool.holders, self.rows
         for s in slots:
-            page = self._open_page(s, lengths[s])
-            if page is not None:
-                writers[page] = writers.get(page, 0) + 1
-        return sum(min(n, self.pool.holders(p) - 1) for p, n in writers.items())
+            length = lengths[s]
+            if length % PAGE_TOKENS:            # (the page is neither empty nor full)
+                row, at = rows[s], length // PAGE_TOKENS
+                if at < len(row) and row[at] >= 0 and holders(row[at]) > 1:
+                    writers.append((s, row[at]))
+                    times[row[at]] = times.get(row[at], 0) + 1
+        return writers, sum(min(n, holders(p) - 1) for p, n in times.items())
 
-    def make_own(self, slots, lengths: dict[int, int]) -> list[tuple[int, int, int]]:
-        """Gives each of ``slots`` a page of its own for the positions behind its length where that page has other holders; the
-        copies this takes, as (source, destination, positions in use)."""
+    def make_own(self, writers, lengths: dict[int, int]) -> list[tuple[int, int, int]]:
+        """Gives each of ``writers`` (see ``shared_writes``) a page of its own while its page has other holders; the copies this takes, as (source,
+        destination, positions in use)."""
         moves = []
-        for s in slots:
-            page = self._open_page(s, lengths[s])
-            if page is not None and self.pool.holders(page) > 1:
+        for s, page in writers:
+            if self.pool.holders(page) > 1:
                 own = self.pool.alloc(1)[0]
                 self.pool.free([page])
                 self.rows[s][lengths[s] // PAGE_TOKENS] = own
                 self._changed(s)
                 moves.append((page, own, lengths[s] % PAGE_TOKENS))
         return moves
-
-    def _open_page(self, slot: int, length: int) -> int | None:
-        """The page that is neither empty nor full, if there is one."""
-        row, at = self.rows[slot], length // PAGE_TOKENS
-        return row[at] if length % PAGE_TOKENS and at < len(row) and row[at] >= 0 else None
 
     def commit(self, slot: int, new_length: int) -> None:
         """The sequence now holds ``new_length`` tokens: let go of pages no later query can reach."""
@@ -501,8 +500,8 @@ class SequenceCache:
                 raise CacheError(f"slot {slot} is not live")
         lengths = self._length
         growing = []            # per paged group, the (slot, new length) that need more pages
-        shared = [g for g in self.paged_groups if g.pool.n_shared]
-        writers = list(dict.fromkeys(slot for slot, n_new in requests if n_new > 0)) if shared else []
+        shared = []             # the groups with pages to copy, and who writes into them
+        slots = None
         for g in self.paged_groups:
             more, n = [], 0
             for slot, n_new in requests:
@@ -511,16 +510,19 @@ class SequenceCache:
                     more.append((slot, lengths[slot] + n_new))
                     n += extra
             if g.pool.n_shared:
-                n += g.shared_writes(writers, lengths)
+                if slots is None:
+                    slots = list(dict.fromkeys(slot for slot, n_new in requests if n_new > 0))
+                writers, copies = g.shared_writes(slots, lengths)
+                n += copies
+                if copies:
+                    shared.append((g, writers))
             if n > g.pool.n_free:
                 raise CacheFull(f"cache group {g.index} needs {n} more page(s) of {PAGE_TOKENS} tokens, "
                                 f"{g.pool.n_free} of {g.pool.n_pages} are free")
             growing.append(more)
-        for g in shared:
-            moves = g.make_own(writers, lengths)
-            if moves:
-                self.ownership_changes += 1
-                g.copy(moves)
+        for g, writers in shared:
+            self.ownership_changes += 1
+            g.copy(g.make_own(writers, lengths))
         for g, more in zip(self.paged_groups, growing):
             for slot, new_length in more:
                 g.reserve(slot, new_length)
