@@ -521,6 +521,8 @@ __device__ __forceinline__ void leave_tile(RowState<D>& st, float* join, int par
 }
 
 // STAGES pages are in shared memory or on their way there.  A piece's parts are joined in the stage that was read last.
+// (The compiler is told how many CTAs share an SM but for wide bfloat16 heads, where it then takes 246 registers in place of 168 and the 4 groups of
+// 4 beams above 36.2 us in place of 34.4.)
 template <typename E, int D, int STAGES>
 __global__ void __launch_bounds__(kBaThreads, sizeof(E) == 4 || D <= 64 ? BeamTile<E, D>::kResident : 0) attention_beams_kernel(const __grid_constant__ BeamAttnArgs a) {
     using T = BeamTile<E, D>;
