@@ -256,11 +256,13 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
         for (int e = 0; e < kBeamEach; ++e) sum[e & 1] += exp2_fast((x[e] - zero) * 1.4426950408889634f);
         total += (double)(sum[0] + sum[1]);
 
+        int reached = 0;            // the list's length behind this thread's candidates
         if (mine >= border) {
             unsigned hits = 0;
 #pragma unroll
             for (int e = 0; e < kBeamEach; ++e) hits |= x[e] >= border ? 1u << e : 0u;
             int at = atomicAdd(&sh.n, __popc(hits));
+            reached = at + __popc(hits);
             for (; hits; hits &= hits - 1) {
                 const int e = __ffs(hits) - 1;
                 float v = x[0];
@@ -269,8 +271,8 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
                 sh.list[at++] = beam_key(v + 0.f, base + place(e));      // (-0 counts as 0)
             }
         }
-        __syncthreads();
-        if (sh.n > limit) border = fmaxf(border, from_rising_bits(cut_down(sh, keep)));
+        // (the barrier itself says whether the list is too long: sh.n, read behind it, may be the next tile's already, whose first threads do not wait)
+        if (__syncthreads_or(reached > limit)) border = fmaxf(border, from_rising_bits(cut_down(sh, keep)));
     }
     {
         const float r = warp_max(ref);

@@ -1,0 +1,41 @@
+"""A beam search's selection where its threads go on at different times: the same call gives the same bits however often it is made."""
+import pytest
+import torch
+
+from gpullama3.java_b200.kernels import ops
+from test_gpu_beam_kernels import _check_selection, _logits, _scores
+
+pytestmark = pytest.mark.gpu
+
+
+def _repeated(logits, scores, n, times):
+    """The selection, and how many of ``times`` more calls (recorded, one after the other) differ from it in any bit."""
+    G = scores.shape[0]
+    outs = lambda: (torch.empty(G, n, device="cuda"), *(torch.empty(G, n, dtype=torch.int32, device="cuda") for _ in range(2)))
+    first, other = outs(), outs()
+    ops.beam_select(logits, scores, *first)
+    words = lambda o: torch.stack([o[0].view(torch.int32), o[1], o[2]])
+    want, differing = words(first), torch.zeros((), dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.beam_select(logits, scores, *other)
+        differing += (words(other) != want).any()
+    for _ in range(times):
+        graph.replay()
+    return first, int(differing)
+
+
+def _rising(rows, V, seed):
+    """Rows that rise with some noise: the candidates of every tile pass those before it, so a list grows over its limit again and again."""
+    return _logits(rows, V, seed=seed, spread=0.5) + torch.arange(V, device="cuda") * (40.0 / V)
+
+
+@pytest.mark.parametrize("make", [_logits, _rising])
+@pytest.mark.parametrize("G, B, V, n", [(8, 32, 128256, 64), (8, 8, 128256, 64), (4, 60, 50257, 200), (2, 150, 90001, 3)])
+def test_rows_of_many_tiles_give_the_same_bits_each_time(G, B, V, n, make):
+    """Each CTA goes through a row in several tiles and cuts its list of candidates down between them, or not."""
+    logits, scores = make(G * B, V, seed=V), _scores(G, B, seed=V)
+    first, differing = _repeated(logits, scores, n, 10000 if V * G * B > 8e6 else 2000)
+    assert differing == 0
+    _check_selection(logits, scores, n, first)
