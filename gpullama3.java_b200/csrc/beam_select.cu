@@ -429,19 +429,21 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         if (lane == 0) sh.high[warp] = mine;
         __syncthreads();
         const unsigned w = lane < kMergeWarps ? sh.high[lane] : 0u, high = __reduce_max_sync(0xffffffffu, w);
-        auto reaching = [&](unsigned t, int set) {
+        int set = 0;
+        auto reaching = [&](unsigned t) {
             int n = __reduce_add_sync(0xffffffffu, count_mine(t));
-            if (lane == 0) sh.count[set][warp] = n;         // (two sets of counts in turn: one barrier a count)
+            set ^= 1;               // (two sets of counts in turn, call by call, whichever bits are counted: one barrier a count)
+            if (lane == 0) sh.count[set][warp] = n;
             __syncthreads();
             return (int)__reduce_add_sync(0xffffffffu, lane < kMergeWarps ? sh.count[set][lane] : 0);
         };
         // numbers that differ from the largest in their last 24 bits only: totals within a factor of four or so
         unsigned least = high & 0xff000000u;
         int bit = 23;
-        if (reaching(least, 0) < need) { least = 0; bit = 31; }
+        if (reaching(least) < need) { least = 0; bit = 31; }
         for (; bit >= 0; --bit) {
             const unsigned t = least | (1u << bit);
-            const int n = t <= high ? reaching(t, bit & 1 ^ 1) : 0;
+            const int n = t <= high ? reaching(t) : 0;
             if (n >= need) {
                 least = t;
                 if (n <= need + need / 4) break;

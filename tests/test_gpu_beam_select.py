@@ -39,3 +39,16 @@ def test_rows_of_many_tiles_give_the_same_bits_each_time(G, B, V, n, make):
     first, differing = _repeated(logits, scores, n, 10000 if V * G * B > 8e6 else 2000)
     assert differing == 0
     _check_selection(logits, scores, n, first)
+
+
+@pytest.mark.parametrize("G, B, V, n", [(8, 8, 4000, 16), (40, 4, 1000, 8), (3, 100, 2000, 30), (2, 500, 300, 50), (1, 4, 128256, 8), (8, 16, 128256, 33)])
+@pytest.mark.parametrize("low", [0.5, 8.0, 120.0])
+def test_merges_of_totals_of_all_sizes_give_the_same_bits_each_time(G, B, V, n, low):
+    """Totals from -0.5 down to far below: the search over their bits skips what lies above the largest, so bits are counted in any order of
+    odd and even; all candidates in registers, and in lists that are looked through."""
+    logits = _logits(G * B, V, seed=n, spread=3.0)
+    scores = -low * torch.rand(G, B, generator=torch.Generator().manual_seed(n)).cuda()
+    for shift in (0.0, 0.3, 1.7):
+        first, differing = _repeated(logits, scores - shift, n, 1000)
+        assert differing == 0
+        _check_selection(logits, scores - shift, n, first)
