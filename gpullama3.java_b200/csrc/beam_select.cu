@@ -358,6 +358,7 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
     if (tid == 0) { sh.n = sh.n_active = sh.n_keys = 0; sh.largest = 0; }
     pdl_launch_dependents();
     pdl_wait();
+    __syncthreads();            // (sh.largest grows below)
     const int lists = beams * chunks;       // in the order of beams
     const long long all = (long long)lists * keep;
     const u64* from = in.candidates + (size_t)g * all;

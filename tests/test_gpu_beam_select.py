@@ -52,3 +52,14 @@ def test_merges_of_totals_of_all_sizes_give_the_same_bits_each_time(G, B, V, n, 
         first, differing = _repeated(logits, scores - shift, n, 1000)
         assert differing == 0
         _check_selection(logits, scores - shift, n, first)
+
+
+def test_beams_of_very_unequal_scores_give_the_same_bits_each_time():
+    """The margin of the merge's rough totals follows the largest of the beams' scores, which all warps put together."""
+    logits = _logits(6 * 16, 3000, seed=2)
+    scores = _scores(6, 16, seed=2)
+    scores[:, 11] = -3.0e4                     # one warp's alone
+    scores[3:, 0] = -1.0e7
+    first, differing = _repeated(logits, scores, 24, 5000)
+    assert differing == 0
+    _check_selection(logits, scores, 24, first)
