@@ -16,13 +16,16 @@
 // searches of 32 steps with a barrier each.  (Lists of each warp by itself need no barriers, but then every warp holds `keep`
 // candidates of its own and the ordering at the end is of eight times as many, which took longer than all the rest.)
 //
-// Exponentials are taken in 32 bits, relative to a whole number, added in 32 bits over eight of a thread's logits and in 64 from there on: a
-// row's lse is off by about 2e-8 of itself (measured against 64 bits), and totals are compared in 64 bits, so that two beams'
-// continuations change places only where they are that near to each other.  A score is rounded to 32 bits once, when it is stored.
+// Exponentials are taken in 32 bits, relative to a whole number that no logit so far exceeds by more than 1, added in 32 bits over eight of a
+// thread's logits and in 64 from there on.  In units of 2^-24 an exponential of x - m = -t is off by 2.3 t (the difference, the product with log2 e,
+// that number's rounding) and 4 (the power of two), the additions by 8; weighed by the probabilities t is at most 1 + log V.  So a row's lse is off by
+// at most 2^-24 (2.3 (1 + log V) + 12), 2.5e-6 for 128,256 tokens (absolutely; measured, the selected scores of ordinary rows, -20 or so, are off by 2.7e-8
+// of their norm, their own rounding included).  Totals are compared in 64 bits, so two beams' continuations change places only where they are that near to each other, and
+// none is above its beam's score, whatever the lse is off by.  A score is rounded to 32 bits once, when it is stored.
 //
 // Bound by: HBM in bytes (4 per logit), in fact by the rows' instructions and the merge's chain of barriers.  Measured: 64 rows of
-// 128,256 logits, 16 kept each of 8, 18.8 us of which the reading needs 5.0; 256 rows, 64 kept, 46.6 us of 20.0 (rows 39 us at 3.4 TB/s,
-// issuing in half of all cycles); 4 rows 10.3 us, of which the two launches, the first tile's search and the merge are nearly all.
+// 128,256 logits, 16 kept each of 8, 18.3 us of which the reading needs 5.0; 256 rows, 64 kept, 47.8 us of 20.0 (rows 39 us at 3.4 TB/s,
+// issuing in half of all cycles); 4 rows 10.5 us, of which the two launches, the first tile's search and the merge are nearly all.
 //
 // Rows that have no distribution give no candidates: a beam whose score is not finite (one that does not count, not read at
 // all), a row that holds NaN or +inf, a row of nothing but -inf.  A logit of -inf is never a candidate.  Places for which there is
@@ -245,7 +248,7 @@ beam_rows_kernel(const float* __restrict__ logits, long long ld, const float* __
             }
             border = from_rising_bits(max(least, kRisingMinusInf + 1u));     // -inf is no candidate
         }
-        if (mine > ref + 16.f) {        // (relative to the maximum of the warp's first logits until that is exceeded by far)
+        if (mine > ref + 1.f) {         // (relative to the maximum of the warp's first logits until that is exceeded)
             const float higher = ceilf(mine);
             total = ref > -INFINITY ? brought_to(total, ref, higher) : total;
             ref = higher;
@@ -343,6 +346,7 @@ struct Beam {
     double exact;       // score - log of the row's sum of exponentials (NaN: the row gives none)
     float ref;          // what the sum is relative to
     float base;         // the first, rounded
+    float score;        // which no total exceeds
 };
 
 // 64-bit arithmetic is slow on this chip (a comparison of 80 by 80 totals took 8 us), so candidates are found by rough totals in 32 bits, off by
@@ -390,7 +394,7 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
             if (top > -INFINITY && top < INFINITY && total < (double)INFINITY) base = (double)score - log(total);
         }
         if (lane == 0) {
-            beam_s[b] = Beam{base, top, (float)base};
+            beam_s[b] = Beam{base, top, (float)base, score};
             if (!isnan(base)) atomicMax(&sh.largest, __float_as_uint(fabsf((float)base)));
         }
     }
@@ -404,7 +408,7 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         if (key == 0ull) return 0u;
         const Beam& b = beam_s[beam_of(list)];
         const float t = (key_logit(key) - b.ref) + b.base;
-        return isnan(t) ? 0u : rising_bits(t);
+        return isnan(t) ? 0u : rising_bits(fminf(t, b.score) + 0.f);
     };
     auto exact = [&](u64 key, int list) {
         Candidate c{0ull, -INFINITY, 0, -1};
@@ -414,7 +418,8 @@ beam_merge_kernel(const float* __restrict__ scores, int beams, int chunks, int k
         if (isnan(b.base)) return c;
         c.token = key_token(key);
         c.logit = key_logit(key);
-        c.total = rising_bits(((double)c.logit - (double)b.ref) + b.exact);
+        // (the log sum may be off by so much that a token of probability 1 comes out above its beam's score)
+        c.total = rising_bits(fmin(((double)c.logit - (double)b.ref) + b.exact, (double)b.score));
         return c;
     };
     // what is taken when `least` is what enough rough totals reach: everything that may be exactly as large

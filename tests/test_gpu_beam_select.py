@@ -1,9 +1,12 @@
-"""A beam search's selection where its threads go on at different times: the same call gives the same bits however often it is made."""
+"""A beam search's selection where its threads go on at different times: the same call gives the same bits however often it is made; and how
+far a sum of log probabilities may be off."""
+import math
+
 import pytest
 import torch
 
 from gpullama3.java_b200.kernels import ops
-from test_gpu_beam_kernels import _check_selection, _logits, _scores
+from test_gpu_beam_kernels import HALF_STEP, _check_selection, _logits, _reference, _scores, _select
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +66,37 @@ def test_beams_of_very_unequal_scores_give_the_same_bits_each_time():
     first, differing = _repeated(logits, scores, 24, 5000)
     assert differing == 0
     _check_selection(logits, scores, 24, first)
+
+
+@pytest.mark.parametrize("background", [0.0, 1.0, 4.0])
+@pytest.mark.parametrize("above", [0.0, 15.9])
+def test_log_probabilities_never_rise_and_are_off_by_a_bounded_amount(above, background):
+    """Rows of one peak behind the first tile of a chunk, ``above`` and more above everything before it.
+
+    A row's log sum is off by at most 2.3 (1 + log V) + 12 half steps, absolutely.  Relative to its reference, at most 1 below and never above the
+    row's largest logit rounded up, a logit is -t with t at most 1 + the distance d to the largest, so its exponential is off by t half steps each
+    from the difference, from the product with log2 e and 0.22 from that number's own rounding, by 4 from the power of two, by 8 from the additions in 32
+    bits.  Weighed by the probabilities p, sum p d = entropy - log sum e^-d is at most log V.  The stored score is rounded once."""
+    B, V = 64, 70001
+    logits = _logits(B, V, seed=int(above), spread=background)
+    at = 4096 + 131 * torch.arange(B, device="cuda")              # (second and third tiles)
+    rows = torch.arange(B, device="cuda")
+    logits[rows, at] = logits[:, :4096].amax(dim=1) + above + torch.linspace(0, 25 - above, B, device="cuda")
+    bound = (2.3 * (1 + math.log(V)) + 12) * HALF_STEP
+    for scores in (torch.zeros(1, B, device="cuda"), _scores(1, B, seed=1)):
+        total, _ = _reference(logits, scores, 1)
+        s, b, t = (o.cpu()[0] for o in _select(logits, scores, 2 * B))
+        assert bool((s <= scores.cpu()[0][b.long()]).all())
+        exact = total[0][b.long(), t.long()]
+        assert bool(((s.double() - exact).abs() <= bound + HALF_STEP * exact.abs()).all())
+        assert len(set(zip(b.tolist(), t.tolist()))) == 2 * B
+        # with a beam to itself
+        s, b, t = (o.cpu()[0] for o in _select(logits[7:8], scores[:, 7:8], 3))
+        assert float(s[0]) <= float(scores[0, 7]) and (above == 0.0 or int(t[0]) == int(at[7]))
+
+
+def test_tokens_whose_probability_is_one_are_ordered_by_beam_whatever_zeros_sign():
+    logits = torch.full((4, 9000), -200.0, device="cuda")
+    logits[:, 5000] = torch.tensor([0.0, -0.0, 30.0, -7.0], device="cuda")
+    s, b, t = _select(logits, torch.tensor([[-0.0, 0.0, -0.0, 0.0]], device="cuda"), 4)
+    assert s.tolist() == [[0.0] * 4] and b.tolist() == [[0, 1, 2, 3]] and t.tolist() == [[5000] * 4]
