@@ -52,24 +52,34 @@ class PagePool:
 
     def share(self, pages) -> None:
         """Each of ``pages`` gets one holder more."""
+        pages = list(pages)
         for p in pages:
             if not (0 <= p < self.n_pages) or self._holders[p] == 0:
                 raise CacheError(f"page {p} is not held and cannot be shared")
+        for p in pages:
             self._holders[p] += 1
             if self._holders[p] == 2:
                 self.n_shared += 1
 
     def free(self, pages) -> None:
+        """Each of ``pages`` comes back from one of its holders.  Nothing changes where one of them cannot."""
         pages = list(pages)
-        for p in pages:
-            if not (0 <= p < self.n_pages):
-                raise CacheError(f"page {p} does not belong to this pool of {self.n_pages}")
-            if self._holders[p] == 0:
+        out = []                                      # those that nobody holds any more
+        for i, p in enumerate(pages):
+            if not (0 <= p < self.n_pages) or self._holders[p] == 0:
+                for q in pages[:i]:
+                    self._holders[q] += 1
+                    if self._holders[q] == 2:
+                        self.n_shared += 1
+                if not (0 <= p < self.n_pages):
+                    raise CacheError(f"page {p} does not belong to this pool of {self.n_pages}")
                 raise CacheError(f"page {p} freed twice")
             self._holders[p] -= 1
             if self._holders[p] == 1:
                 self.n_shared -= 1
-        self._free.extend(p for p in reversed(pages) if self._holders[p] == 0)
+            elif self._holders[p] == 0:
+                out.append(p)
+        self._free.extend(reversed(out))
 
 
 class SlotTable:
