@@ -374,8 +374,9 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const uint32_t (&qa
 
 // float32: x = h + m + l, three bfloat16 numbers of 8 bits each (what is left is below 2^-26 of x); a product is h h + (h m + m h) + (m m + h l + l h),
 // six on the tensor cores with an error below that of one product's rounding.  The three magnitudes are added separately, and the output of 16
-// keys before it joins the row's, in 32 bits: a tensor core's own sum drops bits instead of rounding them.  Numbers from 2^-109 to 2^127 have all three
-// parts; what is not finite gives NaN.
+// keys before it joins the row's, in 32 bits: a tensor core's own sum drops bits instead of rounding them.  Numbers from 2^-109 on have all three
+// parts, smaller ones are held to 2^-134 (half of bfloat16's last place there).  What is not finite, or rounds to infinity in bfloat16 (from 3.39e38 on), gives
+// NaN wherever it is multiplied, and the rows concerned are computed once more, on multiply-adds, where the pieces are joined.
 struct Parts {
     uint32_t h, m, l;
 };
@@ -757,11 +758,74 @@ __global__ void __launch_bounds__(kBaThreads, sizeof(E) == 4 || D <= 64 ? BeamTi
     leave(u1);
 }
 
+// One row from the keys that it sees and nothing else, in 32 bits: for rows that are not numbers, or have no weight, in what the tiles left.  There
+// a number that is not finite (in float32, one that has no parts) comes to NaN in rows that do not see it too, as 0 times itself.
+// By a warp, a lane a key of 32 at a time, then a lane D / 32 dimensions.  q_s: D floats of the warp's own.  (Slow: where all rows of 64 sequences of 3,900
+// positions with 32 heads of 64 are such, 6.7 ms, 9.6 in float32.  A call without such rows takes as long as it did without this.)
+template <typename T, int D>
+__device__ __noinline__ void attend_row(const BeamAttnArgs& a, int seq, int head, float* q_s) {
+    constexpr int E = D / 32, kEach = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31, kvh = head / (a.n_heads / a.n_kv_heads);
+    const int len = a.kv_lens[seq], end = min(len, a.table_stride * kPageTokens), lo = first_key(len, a.window);
+    const T* q = (const T*)a.q + (size_t)seq * a.q_row_stride + (size_t)head * D;
+    for (int d = lane; d < D; d += 32) {
+        float x = to_f32<T>(q[d]);
+        if (a.inv_freq) {               // (as in the tiles: see `turned`)
+            const int j = a.pairing == 0 ? d / 2 : d % (D / 2);
+            const bool second = a.pairing == 0 ? d % 2 != 0 : d >= D / 2;
+            const float other = to_f32<T>(q[a.pairing == 0 ? d ^ 1 : (d + D / 2) % D]);
+            float sn, cs;
+            sincosf((float)(len - 1) * a.inv_freq[j], &sn, &cs);
+            x = to_f32<T>(from_f32<T>(second ? __fmaf_rn(other, sn, __fmul_rn(x, cs)) : __fmaf_rn(x, cs, -__fmul_rn(other, sn))));
+        }
+        q_s[d] = x;
+    }
+    __syncwarp();
+    const float scale = 1.f / sqrtf((float)D);
+    const size_t page_elements = (size_t)a.n_kv_heads * kPageTokens * D, head_off = (size_t)kvh * kPageTokens * D;
+    float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int k0 = lo / 32 * 32; k0 < end; k0 += 32) {
+        const size_t page = (size_t)a.page_table[(size_t)seq * a.table_stride + k0 / kPageTokens] * page_elements + head_off;
+        const int at = k0 % kPageTokens, key = k0 + lane;
+        const bool seen = key >= lo && key < end;
+        float s = -INFINITY;
+        if (seen) {
+            const uint4* k = reinterpret_cast<const uint4*>((const T*)a.k_pool + page + (size_t)(at + lane) * D);
+            s = 0.f;
+#pragma unroll 4
+            for (int c = 0; c < D / kEach; ++c) {
+                const uint4 w = k[c];
+                const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) s = fmaf(q_s[c * kEach + i], to_f32<T>(x[i]), s);
+            }
+            s *= scale;
+        }
+        const float top = fmaxf(m, warp_max(s)), base = top == -INFINITY ? 0.f : top;
+        const float keep = expf(m - base), p = seen ? expf(s - base) : 0.f;
+        m = top;
+        l = l * keep + warp_sum(p);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= keep;
+        const T* v = (const T*)a.v_pool + page + (size_t)lane * kPageTokens + at;
+        for (int i = max(lo - k0, 0); i < min(32, end - k0); ++i) {
+            const float w = __shfl_sync(0xffffffffu, p, i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(w, to_f32<T>(v[(size_t)e * 32 * kPageTokens + i]), o[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) ((T*)a.out)[((size_t)seq * a.n_heads + head) * D + e * 32 + lane] = from_f32<T>(o[e] / l);
+}
+
 // A warp per (sequence, query head): the pieces that hold the row, first those of the shared pages, then of its own.  A lane reads a piece's maximum
 // and sum; the outputs are asked for eight pieces at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_constant__ BeamAttnArgs a, int n_ctas) {
     constexpr int E = D / 32, kAtOnce = 8;
+    __shared__ float q_s[4][D];         // (of rows that are computed once more)
     const int lane = threadIdx.x & 31, at = blockIdx.x * 4 + (threadIdx.x >> 5), rep = a.n_heads / a.n_kv_heads;
     const int seq = at / a.n_heads, head = at - seq * a.n_heads, kvh = head / rep, in_group = head - kvh * rep;
     const int g = seq / a.beams, beam = seq - g * a.beams, sub = a.n_sub == 1 ? 0 : beam / a.sub_beams, i = beam - sub * a.sub_beams;
@@ -820,6 +884,13 @@ __global__ void __launch_bounds__(128) attention_beams_join_kernel(const __grid_
                 for (int e = 0; e < E; ++e) o[e] += v[k][e] * w;
             }
         }
+    }
+    bool lost = n > 0 && !(l > 0.f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) lost = lost || isnan(o[e]);
+    if (__any_sync(0xffffffffu, lost)) {
+        attend_row<T, D>(a, seq, head, q_s[threadIdx.x >> 5]);
+        return;
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;      // (a sequence without keys: zeros)
 #pragma unroll

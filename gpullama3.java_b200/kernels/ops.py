@@ -1372,7 +1372,9 @@ def attention_decode_beams(q: torch.Tensor, q_row_stride: int, out: torch.Tensor
     """``attention_decode`` for sequences in groups of equal size that share their first pages (the beams of a request): group g is
     sequences g B .. (g + 1) B - 1, and the first shared_pages[g] entries of their rows of the page table are the same (int32 [groups]; pages
     that are not full for all of the group's sequences count as each one's own).  ``n_parts``: see ``attention_beams_parts``.  ``plan``: what
-    ``attention_beams_plan`` made of the same lengths, shared pages, heads, window and width of the page table."""
+    ``attention_beams_plan`` made of the same lengths, shared pages, heads, window and width of the page table.  What a sequence does not see
+    counts for nothing, whatever it holds; what it sees may be infinite.  float32 is multiplied in three bfloat16 parts, as exact as float32 from
+    2^-109 on; smaller numbers are held to 2^-134."""
     if out.shape[0] == 0 and shared_pages.numel():
         return
     G, B, scratch = _beams_checked(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan)
