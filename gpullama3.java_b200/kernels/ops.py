@@ -1339,7 +1339,7 @@ def attention_beams_plan(kv_lens: torch.Tensor, shared_pages: torch.Tensor, tabl
     return out
 
 
-def _beams_checked(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan):
+def _beams_checked(q, q_row_stride, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan):
     """The checks that both forms share; the number of groups and of sequences in one, and the scratch."""
     _here(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, scratch, plan)
     n_seqs, n_groups = out.shape[0], shared_pages.numel()
@@ -1350,7 +1350,9 @@ def _beams_checked(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_
     if not attention_beams_takes(n_groups, n_seqs // n_groups, n_heads, n_kv_heads):
         raise KernelError(f"attention_decode_beams: {n_groups} groups of {n_seqs // n_groups} are more than one call takes")
     assert q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and out.is_contiguous() and out.shape[1] == n_heads * head_dim
-    assert q.shape[0] >= n_seqs and q.stride(-1) == 1
+    assert q.dim() == 2 and q.shape[0] >= n_seqs and q.shape[1] >= n_heads * head_dim and q.stride(1) == 1
+    # (the kernel steps from row to row by this number alone)
+    assert n_seqs == 1 or q_row_stride == q.stride(0), f"rows of q lie {q.stride(0)} apart, not {q_row_stride}"
     assert kv_lens.dtype == page_table.dtype == shared_pages.dtype == torch.int32
     assert kv_lens.is_contiguous() and page_table.is_contiguous() and shared_pages.is_contiguous()
     assert kv_lens.numel() == n_seqs and page_table.shape[0] == n_seqs
@@ -1377,8 +1379,8 @@ def attention_decode_beams(q: torch.Tensor, q_row_stride: int, out: torch.Tensor
     2^-109 on; smaller numbers are held to 2^-134."""
     if out.shape[0] == 0 and shared_pages.numel():
         return
-    G, B, scratch = _beams_checked(q, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan)
-    assert q_row_stride >= n_heads * head_dim
+    G, B, scratch = _beams_checked(q, q_row_stride, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts,
+                                   scratch, plan)
     _check(_fn("b200_attention_beams")(
         q.data_ptr(), q_row_stride, out.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), page_table.shape[1], shared_pages.data_ptr(),
         k_pool.data_ptr(), v_pool.data_ptr(), scratch.data_ptr(), scratch.numel(), G, B, n_heads, n_kv_heads, head_dim, int(window),
@@ -1395,7 +1397,8 @@ def attention_decode_beams_rope(qkv: torch.Tensor, out: torch.Tensor, kv_lens: t
     if out.shape[0] == 0 and shared_pages.numel():
         return
     _here(inv_freq)
-    G, B, scratch = _beams_checked(qkv, out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts, scratch, plan)
+    G, B, scratch = _beams_checked(qkv, qkv.stride(0), out, kv_lens, page_table, shared_pages, k_pool, v_pool, n_heads, n_kv_heads, head_dim, n_parts,
+                                   scratch, plan)
     assert qkv.dtype == torch.bfloat16 and qkv.is_contiguous() and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim
     assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.numel() == head_dim // 2
     _check(_fn("b200_attention_beams_rope")(
