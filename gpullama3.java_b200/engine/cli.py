@@ -202,6 +202,9 @@ def main(argv=None) -> int:
 
     if args.beams > 1:
         outs = engine.beam_search(prompts, args.beams, args.max_tokens, length_penalty=args.length_penalty, stop_ids=args.stop)
+        if args.echo:     # (tokens are known when the search is over)
+            for o in outs:
+                print(" ".join(map(str, o)), file=sys.stderr)
     else:
         outs = engine.generate(prompts, max_new_tokens=args.max_tokens, temperature=args.temperature, top_p=args.top_p,
                                seed=seed, stop_ids=args.stop, on_token=on_token)
