@@ -931,16 +931,17 @@ static int fill_args(BeamAttnArgs& a, const int* kv_lens, const int* shared_page
 }
 
 constexpr int kSmShared = 228 * 1024, kCtaShared = 227 * 1024, kCtaReserved = 1024;      // bytes of an SM, the most of a CTA's, what each takes besides
+constexpr int kStaticShared = 16 + kBaRing * (int)sizeof(Unit) + 1024;                      // at most, of attention_beams_kernel
 
 template <typename Kernel>
-static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int), int smem, int (&configured)[64], const BeamAttnArgs& a, int n_ctas,
+static int launch_beams(Kernel kernel, void (*join)(const BeamAttnArgs, int), int smem, bool (&configured)[64], const BeamAttnArgs& a, int n_ctas,
                         cudaStream_t stream) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
-    if (configured[device] < smem) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (!configured[device]) {          // the most that any call takes: of two threads that set it at once neither takes it back
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCtaShared - kStaticShared);
         if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
-        configured[device] = smem;
+        configured[device] = true;
     }
     const int st = launch_pdl(kernel, dim3(n_ctas, a.n_kv_heads), dim3(kBaThreads), smem, stream, a);
     if (st != 0) return st;
@@ -958,13 +959,12 @@ static int beam_smem(const BeamAttnArgs& a, int stages) {
 template <typename E, int D>
 static int launch_beams_of(const BeamAttnArgs& a, int n_ctas, cudaStream_t stream) {
     using T = BeamTile<E, D>;
-    static int configured[2][64] = {};
-    constexpr int kStatic = 16 + kBaRing * (int)sizeof(Unit) + 1024;
+    static bool configured[2][64] = {};
     const auto join = attention_beams_join_kernel<E, D>;
     const int smem = beam_smem<E, D>(a, T::kMore), fewer = beam_smem<E, D>(a, 2);
-    if (smem + kStatic + kCtaReserved <= kSmShared / T::kResident)
+    if (smem + kStaticShared + kCtaReserved <= kSmShared / T::kResident)
         return launch_beams(attention_beams_kernel<E, D, T::kMore>, join, smem, configured[0], a, n_ctas, stream);
-    if (fewer + kStatic > kCtaShared) return kErrUnsupportedSize;
+    if (fewer + kStaticShared > kCtaShared) return kErrUnsupportedSize;
     return launch_beams(attention_beams_kernel<E, D, 2>, join, fewer, configured[1], a, n_ctas, stream);
 }
 template <int D>
