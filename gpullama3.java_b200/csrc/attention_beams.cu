@@ -998,16 +998,9 @@ extern "C" int b200_attention_beams_plan(int* plan, const int* kv_lens, const in
     if (((uintptr_t)plan & 15) != 0) return kErrUnsupportedSize;
     a.plan = plan;
     a.fresh = fresh != 0;
-    static bool configured[64] = {};
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return kErrBadArgument;
-    const int smem = plan_ints(a) * 4;
-    if (smem > 48 * 1024 && !configured[device]) {
-        const cudaError_t e = cudaFuncSetAttribute(attention_beams_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCtaShared - 1024);
-        if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
-        configured[device] = true;
-    }
-    return launch_pdl(attention_beams_plan_kernel, dim3(1), dim3(256), smem, stream, a);
+    // (segments are parts and sequences together, and a part has a sequence at least: sequences and parts twice are at most half as many again)
+    static_assert((4 * (kBaMaxSegments + 1) + 3 * kBaMaxSegments / 2) * 4 <= 48 * 1024, "a plan fits the shared memory that needs no asking");
+    return launch_pdl(attention_beams_plan_kernel, dim3(1), dim3(256), plan_ints(a) * 4, stream, a);
 }
 
 namespace b200 {

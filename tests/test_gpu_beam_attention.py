@@ -149,3 +149,16 @@ def test_float32_attention_of_the_smallest_queries(power):
     g.q, g.k = g.q * 2.0 ** power, g.k * 2.0 ** -power
     off = 64 * 2.0 ** (-134 - power) * keys / 8
     assert float((g.run() - want).abs().max()) <= (2 * math.expm1(2 * off) + 1e-5) * values
+
+
+@pytest.mark.parametrize("G, B", [(1024, 1), (512, 3), (31, 64)])
+def test_plans_of_the_most_groups_that_a_call_takes(G, B):
+    """2,048 segments of pages or nearly: as many groups of one sequence, of three, of 64."""
+    lens = [65 + (37 * i) % 90 for i in range(G * B)]
+    g = Groups([1] * G, lens, 1, 1, 32, torch.bfloat16, seed=G)
+    assert ops.attention_beams_takes(G, B, 1, 1) and not ops.attention_beams_takes(G + 1, B, 1, 1)
+    direct, out = g.run(parts=300), torch.empty(G * B, 32, dtype=torch.bfloat16, device="cuda")
+    plan = ops.attention_beams_plan(g.lens, g.shared, g.width, 1, 1, 0)
+    ops.attention_decode_beams(g.q, g.q.stride(0), out, g.lens, g.table, g.shared, g.k, g.v, 1, 1, 32, 0, 300, plan=plan)
+    assert torch.equal(out, direct)
+    g.check(parts=300)
