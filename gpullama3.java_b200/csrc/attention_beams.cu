@@ -22,8 +22,8 @@
 // Groups of more than 64 rows to a kv head are cut into equal groups of whole beams, each of which reads the shared pages.
 //
 // Bound by HBM in bytes: every key and value that some row reads, once.  Measured (both kernels, no plan given): 4 groups of 4 beams, 32 heads
-// on 8 of 128, at 2,200 to 16,200 positions, 155 MB in 34.4 us, 5.5 TB/s while the pages stream; 8 groups of 8 beams, 32 heads on 8 of 64, at about
-// 4,100 positions, 76 MB in 28.0 us: 2 us for the line, 1.5 until the first page is there, 17 of pages, 4.5 for the join and the rest for starts
+// on 8 of 128, at 2,200 to 16,200 positions, 155 MB in 35.5 us, 5.4 TB/s while the pages stream; 8 groups of 8 beams, 32 heads on 8 of 64, at about
+// 4,100 positions, 76 MB in 29.5 us: 2 us for the line, 1.5 until the first page is there, 20 of pages, 4.5 for the join and the rest for starts
 // and ends; one group of 4 at 920 positions 8.6 us, of which the pages need 0.3.  float32 is bound by the tensor cores (six products for one, 57% of
 // their rate while pages stream): 8 groups of 8 beams, 32 heads on 8 of 64, at about 3,900 positions, 144 MB in 72 us (178 us on
 // multiply-adds, bound by reading queries and probabilities from shared memory).
@@ -288,9 +288,7 @@ struct RowState {
     }
 };
 
-// NK keys of a page, from its key `first` on, for the tile whose query fragments are qa.  Nothing is rescaled unless some row's maximum has grown.  (To
-// let it grow by 2^8 before it is followed saves 0.7 us of 28, and costs bits: a row's largest weight is then rounded like any other, where it
-// is exactly 1 otherwise; against 64 bits 2.2e-3 of the norm in place of 1.8e-3, the rounding of the results alone being 1.7e-3.)
+// NK keys of a page, from its key `first` on, for the tile whose query fragments are qa.  Nothing is rescaled unless some row's maximum has grown.
 template <int D, int NK>
 __device__ __forceinline__ void attend_keys(RowState<D>& st, const uint32_t (&qa)[D / 16][4], uint32_t k_base, uint32_t v_base, int first, int lane,
                                             float scale_log2, bool masked, int position, const int (&row_lo)[2], int row_end) {
@@ -356,16 +354,24 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const uint32_t (&qa
     const uint32_t v_row = v_base + (uint32_t)(row * T::kPitchV);
 #pragma unroll
     for (int kk = 0; kk < NK / 16; ++kk) {
-        // Probabilities are rounded to bfloat16 for the tensor cores, as the values are stored.  Their sum is that of the rounded ones (in 32 bits,
-        // a product with ones): what rounding adds to the weight of a key, it then adds to the sum as well.
+        // A probability goes to the tensor cores as two bfloat16 numbers, what it rounds to and what that leaves, 16 bits together; their sum, a product with
+        // ones in 32 bits, is what it is divided by.  (In one number of 8 bits results are off by 1.7e-3 to 1.8e-3 of their norm against 64 bits, as
+        // they are by 1.65e-3, their own rounding, and 8 groups of 8 beams at 4,100 positions take 26.1 us in place of 29.5, a step of theirs 1.42 ms
+        // in place of 1.47.)
         const uint32_t pa[4] = {pack2(s[2 * kk][0], s[2 * kk][1]), pack2(s[2 * kk][2], s[2 * kk][3]),
                                 pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+        auto left = [&](uint32_t h, float x, float y) { return pack2(x - __uint_as_float(h << 16), y - __uint_as_float(h & 0xffff0000u)); };
+        const uint32_t pr[4] = {left(pa[0], s[2 * kk][0], s[2 * kk][1]), left(pa[1], s[2 * kk][2], s[2 * kk][3]),
+                                left(pa[2], s[2 * kk + 1][0], s[2 * kk + 1][1]), left(pa[3], s[2 * kk + 1][2], s[2 * kk + 1][3])};
+        mma_bf16(st.l, pr, 0x3f803f80u, 0x3f803f80u);
         mma_bf16(st.l, pa, 0x3f803f80u, 0x3f803f80u);
         const uint32_t piece = (uint32_t)((((first >> 3) + kk * 2 + half) ^ low) << 4);
 #pragma unroll
         for (int j = 0; j < D / 8; j += 2) {
             uint32_t vb[4];
             ldmatrix4(vb, v_row + piece + (uint32_t)(j * 8 * T::kPitchV));
+            mma_bf16(st.o[j], pr, vb[0], vb[1]);
+            mma_bf16(st.o[j + 1], pr, vb[2], vb[3]);
             mma_bf16(st.o[j], pa, vb[0], vb[1]);
             mma_bf16(st.o[j + 1], pa, vb[2], vb[3]);
         }
@@ -522,8 +528,8 @@ __device__ __forceinline__ void leave_tile(RowState<D>& st, float* join, int par
 }
 
 // STAGES pages are in shared memory or on their way there.  A piece's parts are joined in the stage that was read last.
-// (The compiler is told how many CTAs share an SM but for wide bfloat16 heads, where it then takes 246 registers in place of 168 and the 4 groups of
-// 4 beams above 36.2 us in place of 34.4.)
+// (The compiler is told how many CTAs share an SM but for wide bfloat16 heads, where it then takes 248 registers in place of 182 and the 4 groups of
+// 4 beams above 37.6 us in place of 35.8.)
 template <typename E, int D, int STAGES>
 __global__ void __launch_bounds__(kBaThreads, sizeof(E) == 4 || D <= 64 ? BeamTile<E, D>::kResident : 0) attention_beams_kernel(const __grid_constant__ BeamAttnArgs a) {
     using T = BeamTile<E, D>;
@@ -759,7 +765,8 @@ __global__ void __launch_bounds__(kBaThreads, sizeof(E) == 4 || D <= 64 ? BeamTi
 }
 
 // One row from the keys that it sees and nothing else, in 32 bits: for rows that are not numbers, or have no weight, in what the tiles left.  There
-// a number that is not finite (in float32, one that has no parts) comes to NaN in rows that do not see it too, as 0 times itself.
+// a number that is not finite (in float32, one that has no parts) comes to NaN in rows that do not see it too, as 0 times itself, and in rows that do, as
+// it meets the parts of a probability one by one.
 // By a warp, a lane a key of 32 at a time, then a lane D / 32 dimensions.  q_s: D floats of the warp's own.  (Slow: where all rows of 64 sequences of 3,900
 // positions with 32 heads of 64 are such, 6.7 ms, 9.6 in float32.  A call without such rows takes as long as it did without this.)
 template <typename T, int D>

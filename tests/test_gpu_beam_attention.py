@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from gpullama3.java_b200.kernels import ops
-from test_gpu_beam_kernels import HALF_STEP, Groups
+from test_gpu_beam_kernels import HALF_STEP, SHAPES, Groups
 
 pytestmark = pytest.mark.gpu
 INF = math.inf
@@ -16,8 +16,9 @@ def _definition(g: Groups, window=0, absolute=0.0):
     """Results in 64 bits from what each sequence sees alone, and how far a kernel may be from them where they are finite.
 
     A score of D products is off by (D + 8) half steps of the sum of their sizes, a probability by as much of itself, twice over with its maximum's;
-    sums over n keys by n half steps, those over blocks of 32 and pieces by 4 each.  bfloat16 probabilities and results: 2^-8 each, the power
-    of two 2^-21.  ``absolute``: of the numbers that went in."""
+    sums over n keys by n half steps, those over blocks of 32 and pieces by 4 each.  bfloat16: a probability is two numbers of 8 bits, so half a step
+    of 2^-9 of what is left after as much, twice with the sum's, its power of two 2^-21; a result half a step, 2^-8.  ``absolute``: of the
+    numbers that went in."""
     rep, low = g.H // g.KVH, g.dtype == torch.bfloat16
     want, bound = torch.zeros(len(g.kv_lens), g.H * g.D, dtype=torch.float64), torch.zeros(len(g.kv_lens), g.H * g.D, dtype=torch.float64)
     for r, n in enumerate(g.kv_lens):
@@ -35,7 +36,7 @@ def _definition(g: Groups, window=0, absolute=0.0):
             seen = q.abs() @ k.abs().T
             seen = seen[torch.isfinite(seen)]
             e = (g.D + 8) * HALF_STEP * float(seen.max() if seen.numel() else 0.0) / math.sqrt(g.D)
-            rel = 2 * e + (n - lo + n / 8 + 80) * HALF_STEP + (2.0 ** -8 + 2.0 ** -21 if low else 4 * HALF_STEP)
+            rel = 2 * e + (n - lo + n / 8 + 80) * HALF_STEP + (2.0 ** -17 + 2.0 ** -21 if low else 4 * HALF_STEP)
             want[r, heads] = w.reshape(-1)
             bound[r, heads] = (rel * (sizes + w.abs()) + (2.0 ** -8 if low else HALF_STEP) * w.abs() * (1 + rel) + absolute + 1e-30).reshape(-1)
     return want, bound
@@ -49,6 +50,13 @@ def _check(g: Groups, window=0, parts=None, absolute=0.0):
     err = (got[finite] - want[finite]).abs()
     assert bool((err <= bound[finite]).all()), float((err / bound[finite]).nan_to_num(INF).max())
     return finite
+
+
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_probabilities_of_bfloat16_attention_are_not_rounded_to_it(case):
+    shared, lens, H, KVH, D = SHAPES[case]
+    g = Groups(shared, lens, H, KVH, D, torch.bfloat16, seed=case + 50, spread=0.5)
+    assert bool(_check(g).all()) and bool(_check(g, window=100).all())
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
