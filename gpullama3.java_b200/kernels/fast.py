@@ -76,9 +76,12 @@ def beams_share_attention(ctx, mixer, dtype, capacity: int) -> bool:
 
     bfloat16: up to 16 sequences the products of a step stream through L1, and the attention of groups, which keeps its pages in shared memory,
     makes every SM change its split twice a layer; beyond that the separate sequences' kernel is faster while they are short, for their pages
-    are in L2 for all but the first of a group.  A step in ms, of groups / of separate sequences: 1B shape 4 beams at 1,000 positions 1.02 / 0.74;
-    5 x 4 at 450 0.98 / 0.95, at 900 0.99 / 1.01, at 1,900 1.05 / 1.13; 8 x 8 at 450 1.22 / 1.16, at 900 1.24 / 1.27, at 4,000 1.42 / 1.98;
-    32 x 2 at 900 1.37 / 1.30, at 1,900 1.52 / 1.58; 8B shape 8 x 8 at 220 4.55 / 4.45, at 900 4.63 / 5.21, at 3,000 5.03 / 7.92.
+    are in L2 for all but the first of a group, and the shorter the wider the heads.  A step in ms, of groups / of separate sequences: 1B shape (heads
+    of 64) 4 beams at 1,000 positions 1.00 / 0.74; 5 x 4 at 600 1.02 / 0.97, at 1,100 1.03 / 1.02, at 1,500 1.06 / 1.07, at 1,900 1.07 / 1.12; 4 x 8 at
+    600 1.06 / 1.10; 8 x 8 at 600 1.26 / 1.18, at 900 1.27 / 1.27, at 1,100 1.30 / 1.32, at 1,900 1.35 / 1.51, at 4,000 1.47 / 1.98; 32 x 2 at 1,100 1.43 /
+    1.35, at 1,900 1.55 / 1.57, at 3,500 1.79 / 1.97; 8B shape (of 128) 8 x 8 at 220 4.60 / 4.41, at 600 4.69 / 4.74, at 900 4.76 / 5.21, at 3,000 5.16 /
+    7.92; 5 x 4 at 600 3.81 / 3.82, at 900 3.77 / 4.07; 32 x 2 at 900 5.03 / 5.36, at 1,500 5.35 / 6.34.  The capacity of a recorded step is a power of two:
+    heads of 64 change over at 1,025 positions (2 beams 2,049), heads of 128 at 513 (2 beams 1,025).
 
     float32: faster as soon as there is enough to read, whatever the number of sequences.  1B shape: 1 x 4 at 900 1.51 / 1.45; 1 x 8 at 1,900 1.99 /
     2.06; 4 x 4 at 450 2.66 / 2.57, at 900 2.69 / 2.73, at 3,900 2.87 / 3.92; 8 x 4 at 200 2.72 / 2.71, at 450 2.78 / 2.84; 8 x 8 at 200
@@ -90,7 +93,7 @@ def beams_share_attention(ctx, mixer, dtype, capacity: int) -> bool:
     if dtype == torch.float32:
         enough = ctx.n_seqs * seen >= 16384
     else:
-        enough = ctx.n_seqs > 16 and seen >= 1024 and beams * capacity >= 4096
+        enough = ctx.n_seqs > 16 and seen * mixer.head_dim >= 1024 * 128 and beams * capacity * mixer.head_dim >= 4096 * 128
     return (enough and ops.attention_beams_supported(dtype, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim)
             and ops.attention_beams_takes(ctx.n_seqs // beams, beams, mixer.n_heads, mixer.n_kv_heads))
 
