@@ -75,13 +75,16 @@ def beams_share_attention(ctx, mixer, dtype, capacity: int) -> bool:
     mixer whose mask is causality and at most a window, where that is faster.  ``capacity``: the longest sequence the step must be right for.
 
     bfloat16: up to 16 sequences the products of a step stream through L1, and the attention of groups, which keeps its pages in shared memory,
-    makes every SM change its split twice a layer; beyond that the separate sequences' kernel is faster while they are short, for their pages
+    makes every SM change its split twice a layer, which pays where positions are many; beyond that the separate sequences' kernel is faster while they are short, for their pages
     are in L2 for all but the first of a group, and the shorter the wider the heads.  A step in ms, of groups / of separate sequences: 1B shape (heads
-    of 64) 4 beams at 1,000 positions 1.00 / 0.74; 5 x 4 at 600 1.02 / 0.97, at 1,100 1.03 / 1.02, at 1,500 1.06 / 1.07, at 1,900 1.07 / 1.12; 4 x 8 at
+    of 64) 1 x 4 at 1,000 positions 1.00 / 0.74, at 16,000 1.24 / 0.97, at 60,000 1.46 / 1.62; 1 x 8 at 16,000 1.34 / 1.22, at 30,000 1.44 / 1.60; 4 x 4 at
+    4,000 1.57 / 1.39, at 9,000 1.70 / 1.69, at 16,000 1.88 / 2.07; 2 x 8 at 4,000 1.56 / 1.37, at 9,000 1.67 / 1.67, at 16,000 1.74 / 2.03; 3 x 4 at 16,000
+    1.74 / 1.97; 1 x 16 at 4,000 1.37 / 1.36, at 9,000 1.48 / 1.65; 8 x 2 at 9,000 1.89 / 1.74, at 16,000 2.16 / 2.17; 5 x 4 at 600 1.02 / 0.97, at 1,100 1.03 / 1.02, at 1,500 1.06 / 1.07, at 1,900 1.07 / 1.12; 4 x 8 at
     600 1.06 / 1.10; 8 x 8 at 600 1.26 / 1.18, at 900 1.27 / 1.27, at 1,100 1.30 / 1.32, at 1,900 1.35 / 1.51, at 4,000 1.47 / 1.98; 32 x 2 at 1,100 1.43 /
-    1.35, at 1,900 1.55 / 1.57, at 3,500 1.79 / 1.97; 8B shape (of 128) 8 x 8 at 220 4.60 / 4.41, at 600 4.69 / 4.74, at 900 4.76 / 5.21, at 3,000 5.16 /
+    1.35, at 1,900 1.55 / 1.57, at 3,500 1.79 / 1.97; 8B shape (of 128) 1 x 8 at 16,000 6.59 / 5.88; 4 x 4 at
+    9,000 8.07 / 7.65, at 16,000 8.58 / 9.77; 2 x 8 at 16,000 8.11 / 9.62; 1 x 16 at 9,000 5.57 / 7.54; 8 x 8 at 220 4.60 / 4.41, at 600 4.69 / 4.74, at 900 4.76 / 5.21, at 3,000 5.16 /
     7.92; 5 x 4 at 600 3.81 / 3.82, at 900 3.77 / 4.07; 32 x 2 at 900 5.03 / 5.36, at 1,500 5.35 / 6.34.  The capacity of a recorded step is a power of two:
-    heads of 64 change over at 1,025 positions (2 beams 2,049), heads of 128 at 513 (2 beams 1,025).
+    heads of 64 change over at 1,025 positions (2 beams 2,049), heads of 128 at 513 (2 beams 1,025), 9 to 16 sequences at 8,193, fewer at 32,769.
 
     float32: faster as soon as there is enough to read, whatever the number of sequences.  1B shape: 1 x 4 at 900 1.51 / 1.45; 1 x 8 at 1,900 1.99 /
     2.06; 4 x 4 at 450 2.66 / 2.57, at 900 2.69 / 2.73, at 3,900 2.87 / 3.92; 8 x 4 at 200 2.72 / 2.71, at 450 2.78 / 2.84; 8 x 8 at 200
@@ -93,7 +96,10 @@ def beams_share_attention(ctx, mixer, dtype, capacity: int) -> bool:
     if dtype == torch.float32:
         enough = ctx.n_seqs * seen >= 16384
     else:
-        enough = ctx.n_seqs > 16 and seen * mixer.head_dim >= 1024 * 128 and beams * capacity * mixer.head_dim >= 4096 * 128
+        if ctx.n_seqs > 16:
+            enough = seen * mixer.head_dim >= 1024 * 128 and beams * capacity * mixer.head_dim >= 4096 * 128
+        else:
+            enough = beams > 2 and seen >= (16384 if ctx.n_seqs > 8 else 65536)
     return (enough and ops.attention_beams_supported(dtype, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim)
             and ops.attention_beams_takes(ctx.n_seqs // beams, beams, mixer.n_heads, mixer.n_kv_heads))
 

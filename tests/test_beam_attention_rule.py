@@ -26,6 +26,11 @@ def _shares(heads, groups, beams, positions, dtype=torch.bfloat16, window=None):
     (LLAMA_1B, 32, 2, 3500, 1.788, 1.968), (LLAMA_1B, 4, 8, 1100, 1.095, 1.156), (LLAMA_1B, 2, 16, 1100, 1.102, 1.156), (LLAMA_8B, 8, 8, 220, 4.601, 4.414),
     (LLAMA_8B, 8, 8, 600, 4.691, 4.735), (LLAMA_8B, 8, 8, 900, 4.759, 5.207), (LLAMA_8B, 8, 8, 3000, 5.160, 7.921), (LLAMA_8B, 5, 4, 900, 3.772, 4.073),
     (LLAMA_8B, 32, 2, 1500, 5.354, 6.336), (LLAMA_3B, 8, 8, 600, 2.814, 2.980), (LLAMA_3B, 5, 4, 900, 2.216, 2.434),
+    (LLAMA_1B, 1, 4, 16000, 1.240, 0.965), (LLAMA_1B, 1, 4, 60000, 1.462, 1.624), (LLAMA_1B, 1, 8, 16000, 1.336, 1.217), (LLAMA_1B, 2, 8, 4000, 1.559, 1.369),
+    (LLAMA_1B, 2, 8, 9000, 1.665, 1.669), (LLAMA_1B, 2, 8, 16000, 1.741, 2.033), (LLAMA_1B, 4, 4, 4000, 1.567, 1.386), (LLAMA_1B, 4, 4, 16000, 1.878, 2.074),
+    (LLAMA_1B, 3, 4, 16000, 1.735, 1.970), (LLAMA_1B, 1, 12, 9000, 1.408, 1.582), (LLAMA_1B, 1, 16, 9000, 1.480, 1.652), (LLAMA_1B, 8, 2, 9000, 1.886, 1.735),
+    (LLAMA_8B, 2, 8, 4000, 7.424, 6.023), (LLAMA_8B, 2, 8, 16000, 8.108, 9.618), (LLAMA_8B, 4, 4, 4000, 7.566, 6.057), (LLAMA_8B, 4, 4, 16000, 8.579, 9.770),
+    (LLAMA_8B, 3, 4, 9000, 7.433, 7.604), (LLAMA_8B, 1, 16, 9000, 5.569, 7.542), (LLAMA_8B, 1, 8, 16000, 6.585, 5.878),
 ])
 def test_the_faster_one_is_taken(heads, groups, beams, positions, shared, separate):
     assert _shares(heads, groups, beams, positions) == (shared < separate)
