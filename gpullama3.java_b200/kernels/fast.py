@@ -83,8 +83,9 @@ def beams_share_attention(ctx, mixer, dtype, capacity: int) -> bool:
     600 1.06 / 1.10; 8 x 8 at 600 1.26 / 1.18, at 900 1.27 / 1.27, at 1,100 1.30 / 1.32, at 1,900 1.35 / 1.51, at 4,000 1.47 / 1.98; 32 x 2 at 1,100 1.43 /
     1.35, at 1,900 1.55 / 1.57, at 3,500 1.79 / 1.97; 8B shape (of 128) 1 x 8 at 16,000 6.59 / 5.88; 4 x 4 at
     9,000 8.07 / 7.65, at 16,000 8.58 / 9.77; 2 x 8 at 16,000 8.11 / 9.62; 1 x 16 at 9,000 5.57 / 7.54; 8 x 8 at 220 4.60 / 4.41, at 600 4.69 / 4.74, at 900 4.76 / 5.21, at 3,000 5.16 /
-    7.92; 5 x 4 at 600 3.81 / 3.82, at 900 3.77 / 4.07; 32 x 2 at 900 5.03 / 5.36, at 1,500 5.35 / 6.34.  The capacity of a recorded step is a power of two:
-    heads of 64 change over at 1,025 positions (2 beams 2,049), heads of 128 at 513 (2 beams 1,025), 9 to 16 sequences at 8,193, fewer at 32,769.
+    7.92; 5 x 4 at 600 3.81 / 3.82, at 900 3.77 / 4.07; 32 x 2 at 900 5.03 / 5.36, at 1,500 5.35 / 6.34.  So heads of 64
+    change over at 1,025 positions (2 beams 2,049), heads of 128 at 513 (2 beams 1,025), 9 to 16 sequences at 8,193, fewer at 32,769: powers of two, as a
+    recorded step's capacity is one.
 
     float32: faster as soon as there is enough to read, whatever the number of sequences.  1B shape: 1 x 4 at 900 1.51 / 1.45; 1 x 8 at 1,900 1.99 /
     2.06; 4 x 4 at 450 2.66 / 2.57, at 900 2.69 / 2.73, at 3,900 2.87 / 3.92; 8 x 4 at 200 2.72 / 2.71, at 450 2.78 / 2.84; 8 x 8 at 200
@@ -97,9 +98,9 @@ def beams_share_attention(ctx, mixer, dtype, capacity: int) -> bool:
         enough = ctx.n_seqs * seen >= 16384
     else:
         if ctx.n_seqs > 16:
-            enough = seen * mixer.head_dim >= 1024 * 128 and beams * capacity * mixer.head_dim >= 4096 * 128
+            enough = seen * mixer.head_dim > 1024 * 64 and beams * capacity * mixer.head_dim > 4096 * 64
         else:
-            enough = beams > 2 and seen >= (16384 if ctx.n_seqs > 8 else 65536)
+            enough = beams > 2 and seen > (8192 if ctx.n_seqs > 8 else 32768)
     return (enough and ops.attention_beams_supported(dtype, mixer.n_heads, mixer.n_kv_heads, mixer.head_dim)
             and ops.attention_beams_takes(ctx.n_seqs // beams, beams, mixer.n_heads, mixer.n_kv_heads))
 

@@ -9,9 +9,9 @@ from gpullama3.java_b200.kernels import fast
 LLAMA_1B, LLAMA_3B, LLAMA_8B = (32, 8, 64), (24, 8, 128), (32, 8, 128)
 
 
-def _shares(heads, groups, beams, positions, dtype=torch.bfloat16, window=None):
+def _shares(heads, groups, beams, positions, dtype=torch.bfloat16, window=None, recorded=True):
     n_heads, n_kv_heads, head_dim = heads
-    capacity = 256
+    capacity = 256 if recorded else positions + 1       # (a step launched by itself need be right for its own lengths alone)
     while capacity < positions + 1:
         capacity *= 2
     ctx = types.SimpleNamespace(beams=beams, all_decode=True, n_seqs=groups * beams)
@@ -40,3 +40,10 @@ def test_a_window_counts_as_what_is_seen():
     assert _shares(LLAMA_1B, 8, 8, 4000, window=4096) and not _shares(LLAMA_1B, 8, 8, 4000, window=1000)
     assert _shares(LLAMA_8B, 8, 8, 4000, window=1024) and not _shares(LLAMA_8B, 8, 8, 4000, window=500)
     assert _shares(LLAMA_1B, 8, 8, 2000, torch.float32, window=256) and not _shares(LLAMA_1B, 8, 8, 2000, torch.float32, window=255)
+
+
+@pytest.mark.parametrize("heads, groups, beams, last", [(LLAMA_1B, 8, 8, 1023), (LLAMA_1B, 5, 4, 1023), (LLAMA_1B, 32, 2, 2047), (LLAMA_8B, 8, 8, 511), (LLAMA_8B, 32, 2, 1023),
+                                                        (LLAMA_1B, 4, 4, 8191), (LLAMA_8B, 1, 9, 8191), (LLAMA_1B, 1, 8, 32767)])
+def test_recorded_and_launched_steps_change_over_at_the_same_length(heads, groups, beams, last):
+    for recorded in (True, False):
+        assert not _shares(heads, groups, beams, last, recorded=recorded) and _shares(heads, groups, beams, last + 1, recorded=recorded)
